@@ -22,6 +22,7 @@ FLAG_HOST_IO = 256
 FLAG_NO_SYNC = 512
 FLAG_W_FP8 = 2048
 PATH_NONE, PATH_GEMV, PATH_MMA = 0, 1, 2
+BF16, F16, F32 = 0, 1, 2  # element types of the operators around a decode step
 
 class FmmsCall(ctypes.Structure):
     """``fmms_call_t`` of include/fmms_b200.h, field for field."""
@@ -64,6 +65,19 @@ class FmmsCall(ctypes.Structure):
         ("topk_workspace", c_void_p),
         ("topk_workspace_bytes", c_size_t),
         ("w_scale", c_void_p),
+    ]
+
+
+class FmmsBeamState(ctypes.Structure):
+    """``fmms_beam_state_t`` of include/fmms_b200.h, field for field."""
+
+    _fields_ = [
+        ("data", c_void_p),
+        ("beam_stride", c_longlong),
+        ("outer_stride", c_longlong * 2),
+        ("outer", c_int * 2),
+        ("seg_bytes", c_longlong),
+        ("step_bytes", c_longlong),
     ]
 
 
@@ -144,6 +158,31 @@ SIGNATURES = {
             c_void_p, c_void_p,  # status_dev, stream
         ],
     ),
+    "fmms_int4_linear": (
+        c_int,
+        [
+            c_void_p, c_int, c_longlong,  # x, x_dtype, x_stride
+            c_void_p, c_void_p, c_int, c_void_p,  # qweight, scales, scale_dtype, zeros
+            c_int, c_int, c_int, c_int,  # V, D, group, B
+            c_void_p, c_int, c_longlong,  # out, out_dtype, out_stride
+            c_void_p, c_void_p,  # status_dev, stream
+        ],
+    ),
+    "fmms_query_beam_workspace": (c_int, [c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(c_size_t)]),
+    "fmms_beam_step": (
+        c_int,
+        [
+            c_void_p, c_int, c_longlong, c_longlong,  # logits, dtype, stride_r, stride_k
+            c_void_p, c_void_p, c_longlong,  # scores, finished, pad_token
+            c_int, c_int, c_int, c_int,  # R, K, V, N
+            c_void_p, c_void_p, c_void_p,  # out_scores, out_tokens, out_parents
+            c_void_p, c_size_t, c_void_p,  # workspace, workspace_bytes, stream
+        ],
+    ),
+    "fmms_reorder_beams": (
+        c_int,
+        [ctypes.POINTER(FmmsBeamState), c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p],
+    ),
 }
 
 _lib = None
@@ -201,6 +240,12 @@ def query_staging(d: int, b: int, s: int) -> int:
     n = c_size_t(0)
     check(load().fmms_query_staging(d, b, s, ctypes.byref(n)), "fmms_query_staging")
     return int(n.value)
+
+
+def query_beam_workspace(r: int, k: int, v: int, n: int, dtype: int) -> int:
+    nbytes = c_size_t(0)
+    check(load().fmms_query_beam_workspace(r, k, v, n, dtype, ctypes.byref(nbytes)), "fmms_query_beam_workspace")
+    return int(nbytes.value)
 
 
 PLAN_FIELDS = ("path", "grid", "tile_rows", "tiles_per_cta", "stages", "m_tiles", "smem_bytes", "candidate_rows")

@@ -1,7 +1,7 @@
 """Build recipe of the C-ABI CUDA library (sm_100a only).
 
-``python -m flashsampling_b200.build`` compiles ``csrc/fmms_api.cu`` (which
-includes the kernel headers) into ``lib/libfmms_b200.so`` with nvcc.  The
+``python -m flashsampling_b200.build`` compiles ``csrc/fmms_api.cu`` and
+``csrc/fmms_decode.cu`` (which include the kernel headers) into ``lib/libfmms_b200.so`` with nvcc.  The
 shared object is kept in-tree, next to the sources, and loaded with ctypes; it
 links the CUDA runtime statically and needs nothing from PyTorch.
 """
@@ -17,13 +17,15 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "lib" / "libfmms_b200.so"
-SOURCES = [CSRC / "fmms_api.cu"]
+SOURCES = [CSRC / "fmms_api.cu", CSRC / "fmms_decode.cu"]
 NVCC_FLAGS = [
     "-std=c++17",
     "-O3",
     "-gencode",
     "arch=compute_100a,code=sm_100a",
     "-lineinfo",
+    "--threads",
+    "0",
     "-shared",
     "-Xcompiler",
     "-fPIC",

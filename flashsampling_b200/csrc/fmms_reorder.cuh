@@ -1,0 +1,179 @@
+// Per-beam states after a beam step: beam j of request r goes on with the state of beam parents[r, j].
+//
+//   state[.., r K + j, ..] <- state[.., r K + parents[r, j], ..]      in place, any number of tensors per launch
+//
+// In place because most of the traffic then is what cannot be avoided: a beam that keeps its own state is neither read
+// (unless another one takes it) nor written, and nothing is copied back.  It needs no buffer and no order between
+// threads: a thread owns one column (up to 16 bytes at one offset of all K beams of a request), reads it for every beam
+// that changes, and only then writes.  Positions at or behind a request's length are neither read nor written.
+#pragma once
+
+#include "fmms_common.cuh"
+
+namespace fmms {
+
+constexpr int kReorderThreads = 256;
+constexpr int kReorderMaxStates = 64;     // tensors per launch
+constexpr int kReorderMaxRequests = 1024;  // requests per launch
+constexpr int kReorderMaxBeams = 64;
+
+struct ReorderState {
+  uint8_t* data;
+  long long beam_stride;      // bytes from beam to beam
+  long long outer_stride[2];  // bytes; the two outer dimensions around the beams
+  int outer[2];
+  long long seg_bytes;        // contiguous bytes of a beam at one outer index
+  long long step_bytes;       // bytes of one position, 0: the state has no positions
+  int vec;                    // bytes of a column: divides all of the above and the address
+};
+
+struct ReorderParams {
+  ReorderState st[kReorderMaxStates];
+  const void* parents;        // [R, K] int64 or int32
+  const int* lengths;         // [R] or null
+  int parents_wide;
+  int R, K;
+};
+
+template <int VEC>
+struct ReorderVec;
+template <>
+struct ReorderVec<16> { using type = uint4; };
+template <>
+struct ReorderVec<8> { using type = uint2; };
+template <>
+struct ReorderVec<4> { using type = uint32_t; };
+template <>
+struct ReorderVec<2> { using type = uint16_t; };
+template <>
+struct ReorderVec<1> { using type = uint8_t; };
+
+__device__ __forceinline__ int reorder_parent(const ReorderParams& p, int r, int j) {
+  const size_t at = (size_t)r * p.K + j;
+  const long long v = p.parents_wide ? reinterpret_cast<const long long*>(p.parents)[at]
+                                     : (long long)reinterpret_cast<const int*>(p.parents)[at];
+  return (v < 0 || v >= p.K) ? j : (int)v;  // not a beam of the request: keep the own state
+}
+
+// The columns of one tensor.  KM: beams rounded up; U: columns a thread handles at a time.
+template <int KM, int U, int VEC>
+__device__ __forceinline__ void reorder_columns(const ReorderParams& p, const ReorderState& s, const int* prefix) {
+  using V = typename ReorderVec<VEC>::type;
+  constexpr int kUnit = kReorderThreads * U;
+  const int tid = threadIdx.x;
+  const long long cols = s.seg_bytes / VEC;
+  const long long outers = (long long)s.outer[0] * s.outer[1];
+
+  auto move = [&](uint8_t* const (&at)[U], const int (&req)[U]) {  // req < 0: nothing to do
+    V v[U][KM];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < KM; ++j)
+        if (req[u] >= 0 && j < p.K) {
+          const int par = reorder_parent(p, req[u], j);
+          if (par != j) v[u][j] = *reinterpret_cast<const V*>(at[u] + par * s.beam_stride);
+        }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < KM; ++j)
+        if (req[u] >= 0 && j < p.K && reorder_parent(p, req[u], j) != j) *reinterpret_cast<V*>(at[u] + j * s.beam_stride) = v[u][j];
+  };
+
+  if (cols >= kUnit / 2) {
+    // long segments: a unit is kUnit columns of one (outer index, request); prefix[r]: live units of the requests below r
+    const int per_outer = prefix[p.R];
+    for (long long unit = blockIdx.x; unit < outers * per_outer; unit += gridDim.x) {
+      const long long o = unit / per_outer;
+      const int i = (int)(unit - o * per_outer);
+      int lo = 0, hi = p.R - 1;  // the last r with prefix[r] <= i
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (prefix[mid] <= i) lo = mid; else hi = mid - 1;
+      }
+      const int r = lo;
+      long long live = cols;
+      if (p.lengths && s.step_bytes) live = min(cols, max(0, p.lengths[r]) * (s.step_bytes / VEC));
+      const long long o0 = o / s.outer[1], o1 = o - o0 * s.outer[1];
+      uint8_t* seg = s.data + o0 * s.outer_stride[0] + o1 * s.outer_stride[1] + (long long)r * p.K * s.beam_stride;
+      uint8_t* at[U];
+      int req[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long col = (long long)(i - prefix[r]) * kUnit + u * kReorderThreads + tid;
+        at[u] = seg + col * VEC;
+        req[u] = col < live ? r : -1;
+      }
+      move(at, req);
+    }
+    return;
+  }
+  // short segments: the columns of all (outer index, request) one after the other
+  const long long total = outers * p.R * cols;
+  for (long long base = (long long)blockIdx.x * kUnit; base < total; base += (long long)gridDim.x * kUnit) {
+    uint8_t* at[U];
+    int req[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long x = base + u * kReorderThreads + tid;
+      req[u] = -1;
+      at[u] = s.data;
+      if (x < total) {
+        const long long seg = x / cols, col = x - seg * cols;
+        const long long o = seg / p.R;
+        const int r = (int)(seg - o * p.R);
+        const long long o0 = o / s.outer[1], o1 = o - o0 * s.outer[1];
+        long long live = cols;
+        if (p.lengths && s.step_bytes) live = min(cols, max(0, p.lengths[r]) * (s.step_bytes / VEC));
+        if (col < live) req[u] = r;
+        at[u] = s.data + o0 * s.outer_stride[0] + o1 * s.outer_stride[1] + (long long)r * p.K * s.beam_stride + col * VEC;
+      }
+    }
+    move(at, req);
+  }
+}
+
+// grid (CTAs per tensor, tensors)
+template <int KM, int U>
+__global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_constant__ ReorderParams p) {
+  __shared__ int prefix[kReorderMaxRequests + 1];
+  const ReorderState& s = p.st[blockIdx.y];
+  constexpr int kUnit = kReorderThreads * U;
+  if (s.seg_bytes / s.vec >= kUnit / 2) {
+    for (int r = threadIdx.x; r < p.R; r += kReorderThreads) {
+      long long live = s.seg_bytes;
+      if (p.lengths && s.step_bytes) live = min(live, max(0, p.lengths[r]) * s.step_bytes);
+      prefix[r + 1] = (int)((live / s.vec + kUnit - 1) / kUnit);
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {  // inclusive sums, 32 at a time
+      int carry = 0;
+      for (int b = 0; b < p.R; b += 32) {
+        const int r = b + threadIdx.x;
+        int v = r < p.R ? prefix[r + 1] : 0;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const int o = __shfl_up_sync(0xffffffffu, v, off);
+          if ((int)threadIdx.x >= off) v += o;
+        }
+        v += carry;
+        if (r < p.R) prefix[r + 1] = v;
+        carry = __shfl_sync(0xffffffffu, v, 31);
+      }
+      if (threadIdx.x == 0) prefix[0] = 0;
+    }
+    __syncthreads();
+  }
+  switch (s.vec) {
+    case 16:
+      if constexpr (KM <= 32) reorder_columns<KM, U, 16>(p, s, prefix);  // 64 beams: columns of at most 8 bytes
+      break;
+    case 8: reorder_columns<KM, U, 8>(p, s, prefix); break;
+    case 4: reorder_columns<KM, U, 4>(p, s, prefix); break;
+    case 2: reorder_columns<KM, U, 2>(p, s, prefix); break;
+    default: reorder_columns<KM, U, 1>(p, s, prefix); break;
+  }
+}
+
+}  // namespace fmms

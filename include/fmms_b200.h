@@ -355,6 +355,85 @@ int fmms_static_max_items(void);
  * again" for callers that own no workspace.  No reference counterpart. */
 int fmms_static_reset(void* stream);
 
+/* ---- operators around a decode step ------------------------------------------------------------
+ *
+ * Products with a head (or any linear layer) held in 4 bits, the selection step of a beam search, and the
+ * reordering of per-beam states that follows it.  No reference counterpart: the reference samples from a bf16
+ * head only (core.py:224-348).
+ */
+
+/* element types of these operators */
+#define FMMS_BF16 0
+#define FMMS_F16 1
+#define FMMS_F32 2
+
+/*
+ * out[b, v] = sum_k x[b, k] * (q[v, k] - z[v, k / group]) * s[v, k / group]
+ *
+ *   x            [B, D] bf16 or fp16, rows `x_stride` elements apart
+ *   qweight      [tiles][chunks][512] bytes, 16-byte aligned: tile = 16 weight rows, chunk = 64 columns; the byte at
+ *                [g 8][t 4][j 4][b1 2][b0 2] holds column 16 j + 8 b0 + 2 t + b1 of rows g (low nibble) and 8 + g
+ *                (high nibble); rows beyond V and columns beyond D may hold anything
+ *   scales       [tiles][D / group][8][2] bf16 or fp16 (rows g and 8 + g next to each other), 16-byte aligned
+ *   zeros        the same shape in uint8, or NULL: 8 everywhere
+ *   group        32, 64, 128 or 256, a divisor of D
+ *   out          [B, V] bf16, fp16 or fp32, rows `out_stride` elements apart; written once, nothing else is touched
+ *
+ * Sums are fp32; x is brought to fp16 with an exact power of two per row (values below 2^-28 of a row's largest
+ * lose bits beyond 2^-39 of it).  A row of x that is not finite gives a row that is not finite.  The order of
+ * additions is fixed: equal calls give equal bits, and a row's result does not depend on the other rows of its
+ * call's batch as long as the number of rows stays within the same of the ranges 1-8, 9-16, 17 and more.
+ */
+int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void* qweight, const void* scales,
+                     int scale_dtype, const void* zeros, int V, int D, int group, int B, void* out, int out_dtype,
+                     long long out_stride, int* status_dev, void* stream);
+
+/*
+ * One step of a beam search.  For each of R requests with K beams: of all continuations (beam k, token v) the N with
+ * the largest scores[r, k] + logits[r, k, v] - ln sum_v exp(logits[r, k, v]), in descending order, equal ones in the
+ * order of (k, v).  Sums and totals are formed in 64 bits.
+ *
+ *   logits       row (r, k) starts at r * stride_r + k * stride_k elements; V consecutive bf16, fp16 or fp32 values.
+ *                NaN and -inf are tokens that may not follow.  A row with +inf, or with nothing above -inf, gives no
+ *                candidate
+ *   scores       [R, K]; a beam whose score is not finite gives no candidate, and its logits are not read
+ *   finished     [R, K] bytes, nullable: a beam with a nonzero byte gives the one candidate (pad_token, its score), and
+ *                its logits are not read
+ *   out_*        [R, N] score, token and beam (0..K-1) of each candidate; where fewer than N exist the rest is
+ *                (-inf, -1, min(position, K - 1))
+ *   workspace    fmms_query_beam_workspace() bytes, 16-byte aligned; holds nothing between calls, need not be zeroed,
+ *                and must not be used by two calls at once
+ *
+ * Limits: N <= 64, K <= 64, N <= K * V < 2^31, R * K <= 65535.
+ */
+int fmms_query_beam_workspace(int R, int K, int V, int N, int dtype, size_t* bytes);
+int fmms_beam_step(const void* logits, int dtype, long long stride_r, long long stride_k, const float* scores,
+                   const unsigned char* finished, long long pad_token, int R, int K, int V, int N, float* out_scores,
+                   long long* out_tokens, long long* out_parents, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/*
+ * state[.., r * K + j, ..] <- state[.., r * K + parents[r, j], ..] for every state, in place: per-beam caches, token
+ * histories and recurrent states after a beam step.
+ *
+ * A state is `outer[0] x outer[1]` blocks of R * K beams (all strides in bytes; a beam lies `beam_stride` behind the
+ * one before), each beam one run of `seg_bytes` contiguous bytes per block.  With `lengths` [R] and step_bytes > 0 the
+ * run is made of positions of step_bytes each, of which the first lengths[r] are moved and the others left as they
+ * are.  parents [R, K] are 4- or 8-byte integers; one outside 0..K-1 keeps the beam's own state.  States must not
+ * overlap, nor the beams of one state.  Limit: K <= 64.
+ */
+typedef struct fmms_beam_state {
+  void* data;
+  long long beam_stride;
+  long long outer_stride[2];
+  int outer[2];
+  long long seg_bytes;
+  long long step_bytes;
+} fmms_beam_state_t;
+
+int fmms_reorder_beams(const fmms_beam_state_t* states, int n_states, const void* parents, int parents_bytes, int R,
+                       int K, const int* lengths, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,231 @@
+"""CPU tests of the operators around a decode step: the 4-bit layout and quantiser, the argument checks of the entry
+points and of the C functions (all before any CUDA call), and the description of states for the reordering."""
+
+import ctypes
+
+import pytest
+import torch
+
+import flashsampling_b200 as fs
+from flashsampling_b200 import _lib, beam
+from flashsampling_b200.quant import quantize_groups_int4
+
+
+def _codes(rows, cols, group, zeros, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(0, 16, (rows, cols), generator=g, dtype=torch.uint8)
+    s = (torch.rand(rows, cols // group, generator=g) + 0.5).to(torch.bfloat16)
+    z = torch.randint(0, 16, (rows, cols // group), generator=g, dtype=torch.uint8) if zeros else None
+    return q, s, z
+
+
+@pytest.mark.parametrize("rows,cols,group,zeros", [(1, 32, 32, False), (16, 64, 64, True), (17, 96, 32, True), (40, 256, 256, False), (33, 384, 128, True)])
+def test_layout_follows_its_description(rows, cols, group, zeros):
+    q, s, z = _codes(rows, cols, group, zeros)
+    w = fs.Int4Weight.from_rows(q, s, z)
+    assert w.shape == (rows, cols) and w.group_size == group
+    flat = w.qweight
+    for r in range(rows):
+        for c in range(0, cols, 7):
+            k = c % 16
+            byte = (r % 8) * 64 + (k % 8 // 2) * 16 + (c % 64 // 16) * 4 + (k % 2) * 2 + k // 8
+            assert int(flat[r // 16, c // 64, byte]) >> (4 * (r % 16 // 8)) & 15 == int(q[r, c])
+            assert w.scales[r // 16, c // group, r % 8, r % 16 // 8] == s[r, c // group]
+            if zeros:
+                assert w.zeros[r // 16, c // group, r % 8, r % 16 // 8] == z[r, c // group]
+    assert torch.equal(w.codes(), q)
+    zero = 8 if z is None else z.double().repeat_interleave(group, 1)
+    assert torch.equal(w.dequantize(torch.float64), (q.double() - zero) * s.double().repeat_interleave(group, 1))
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_quantiser_rounds_to_the_nearest_code(symmetric, dtype):
+    w = (torch.randn(50, 256, generator=torch.Generator().manual_seed(1)) * 0.05).to(dtype)
+    w[3] = 0
+    w[4, :128] = 0.01  # one-sided group
+    q, s, z = quantize_groups_int4(w, 128, symmetric)
+    assert s.dtype == (dtype if dtype != torch.float32 else torch.bfloat16) and (z is None) == symmetric
+    back = fs.Int4Weight.from_rows(q, s, z).dequantize(torch.float64)
+    # half a step, plus what the rounding of the scale (eps / 2 relative, over up to 15 steps) and of the zero point
+    # (half a step) can push beyond the last code
+    step = s.double().repeat_interleave(128, 1)
+    slack = 15 * torch.finfo(s.dtype).eps / 2 + (0 if symmetric else 0.5)
+    assert bool(((back - w.double()).abs() <= step * (0.5 + slack) + 1e-12).all())
+    assert bool((back[3] == 0).all())
+    direct = fs.Int4Weight.quantize(w, 128, symmetric)
+    assert torch.equal(direct.codes(), q)
+
+
+def test_quantiser_refuses():
+    w = torch.randn(4, 96)
+    for bad in (dict(group_size=48), dict(group_size=64), dict(group_size=512)):
+        with pytest.raises(ValueError):
+            quantize_groups_int4(w, **bad)
+    with pytest.raises(TypeError):
+        quantize_groups_int4(w, 32, scale_dtype=torch.float32)
+    with pytest.raises(ValueError):
+        quantize_groups_int4(w[0], 32)
+    with pytest.raises(ValueError):
+        quantize_groups_int4(w.to(torch.int32), 32)
+
+
+def test_int4_weight_refuses_other_layouts():
+    q, s, z = _codes(20, 128, 64, True)
+    w = fs.Int4Weight.from_rows(q, s, z)
+    ok = (w.qweight, w.scales, w.zeros)
+    with pytest.raises(ValueError):
+        fs.Int4Weight(*ok, rows=0, cols=128)
+    with pytest.raises(ValueError):
+        fs.Int4Weight(*ok, rows=40, cols=128)  # another number of tiles
+    with pytest.raises(ValueError):
+        fs.Int4Weight(*ok, rows=20, cols=256)
+    with pytest.raises(ValueError):
+        fs.Int4Weight(w.qweight.to(torch.int8), w.scales, w.zeros, 20, 128)
+    with pytest.raises(TypeError):
+        fs.Int4Weight(w.qweight, w.scales.float(), w.zeros, 20, 128)
+    with pytest.raises(ValueError):
+        fs.Int4Weight(w.qweight, w.scales[:, :1].expand(-1, 3, -1, -1).contiguous(), None, 20, 128)  # 3 groups of 128
+    with pytest.raises(ValueError):
+        fs.Int4Weight(w.qweight, w.scales, w.zeros.float(), 20, 128)
+    with pytest.raises(ValueError):
+        fs.Int4Weight(w.qweight, w.scales.transpose(2, 3), w.zeros, 20, 128)
+    odd = torch.empty(w.qweight.numel() + 1, dtype=torch.uint8)[1:].view(w.qweight.shape)
+    with pytest.raises(ValueError):
+        fs.Int4Weight(odd, w.scales, w.zeros, 20, 128)  # not on a 16-byte boundary
+    with pytest.raises(ValueError):
+        fs.Int4Weight.from_rows(q, s[:10], None)
+    with pytest.raises(ValueError):
+        fs.Int4Weight.from_rows(q, s, z[:, :1])
+    with pytest.raises(TypeError):
+        fs.int4_linear(torch.zeros(1, 128, dtype=torch.bfloat16), w.dequantize())
+    with pytest.raises(RuntimeError, match="CUDA"):
+        fs.int4_linear(torch.zeros(1, 128, dtype=torch.bfloat16), w)
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(RuntimeError, match="CUDA"):
+        fs.beam_search_step(torch.zeros(2, 3, 5), torch.zeros(2, 3))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        fs.reorder_beams(torch.zeros(6, 5), torch.zeros(2, 3, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="GPU"):
+        fs.BeamSearch(torch.zeros(8, 8, dtype=torch.bfloat16), 1, 2, 3)
+
+
+def test_c_entry_points_check_their_arguments(lib):
+    p = 4096  # never dereferenced
+    ok = [p, 0, 64, p, p, 0, None, 100, 64, 64, 2, p, 2, 100, None, None]
+
+    def int4(**kw):
+        names = "x x_dtype x_stride q s s_dtype z V D group B out out_dtype out_stride status stream".split()
+        return lib.fmms_int4_linear(*[kw.get(n, v) for n, v in zip(names, ok)])
+
+    for kw in (dict(x=None), dict(q=None), dict(s=None), dict(out=None), dict(V=0), dict(D=0), dict(B=0), dict(B=-1),
+               dict(x_dtype=2), dict(x_dtype=-1), dict(s_dtype=2), dict(out_dtype=3), dict(x_stride=63), dict(out_stride=99)):
+        assert int4(**kw) == _lib.ERR_BAD_ARG, kw
+    for kw in (dict(group=48), dict(group=128), dict(group=0), dict(q=p + 8), dict(s=p + 2), dict(z=p + 4)):
+        assert int4(**kw) == _lib.ERR_UNSUPPORTED, kw
+
+    n = ctypes.c_size_t()
+    assert lib.fmms_query_beam_workspace(2, 4, 1000, 8, 0, ctypes.byref(n)) == 0 and n.value >= 8 * 8 * 8
+    assert lib.fmms_query_beam_workspace(2, 4, 1000, 8, 3, ctypes.byref(n)) == _lib.ERR_BAD_ARG
+    assert lib.fmms_query_beam_workspace(2, 4, 1000, 65, 0, ctypes.byref(n)) == _lib.ERR_UNSUPPORTED
+    assert lib.fmms_query_beam_workspace(2, 4, 1000, 8, 0, None) == _lib.ERR_BAD_ARG
+    beam_ok = [p, 0, 4000, 1000, p, None, 0, 2, 4, 1000, 8, p, p, p, p, 1 << 20, None]
+
+    def step(**kw):
+        names = "x dtype sr sk scores done pad R K V N os ot op ws wsb stream".split()
+        return lib.fmms_beam_step(*[kw.get(m, v) for m, v in zip(names, beam_ok)])
+
+    for kw in (dict(x=None), dict(scores=None), dict(os=None), dict(ot=None), dict(op=None), dict(R=0), dict(K=0), dict(V=0),
+               dict(N=0), dict(dtype=3), dict(pad=-1), dict(pad=1000), dict(V=1, N=5), dict(x=p + 1), dict(x=p + 2, dtype=2)):
+        assert step(**kw) == _lib.ERR_BAD_ARG, kw
+    for kw in (dict(N=65), dict(K=65), dict(K=64, V=1 << 26), dict(R=1 << 16, K=1)):
+        assert step(**kw) == _lib.ERR_UNSUPPORTED, kw
+    for kw in (dict(ws=None), dict(ws=p + 8), dict(wsb=16)):
+        assert step(**kw) == _lib.ERR_WORKSPACE, kw
+
+    st = (_lib.FmmsBeamState * 1)()
+
+    def reorder(**kw):
+        d = dict(data=p, beam_stride=64, outer=(1, 1), seg_bytes=64, step_bytes=0, states=st, n=1, parents=p, pb=8, R=2, K=4)
+        d.update(kw)
+        st[0].data, st[0].beam_stride, st[0].seg_bytes, st[0].step_bytes = d["data"], d["beam_stride"], d["seg_bytes"], d["step_bytes"]
+        st[0].outer[0], st[0].outer[1] = d["outer"]
+        return lib.fmms_reorder_beams(d["states"], d["n"], d["parents"], d["pb"], d["R"], d["K"], None, None)
+
+    for kw in (dict(states=None), dict(n=0), dict(parents=None), dict(pb=2), dict(R=0), dict(K=0), dict(data=None),
+               dict(outer=(0, 1)), dict(outer=(1, -1)), dict(seg_bytes=0), dict(step_bytes=-1), dict(step_bytes=48)):
+        assert reorder(**kw) == _lib.ERR_BAD_ARG, kw
+    assert reorder(K=65) == _lib.ERR_UNSUPPORTED
+
+
+def _moved(state, desc, R, K, parents, lengths):
+    """What the kernel's addressing does with a described state, on the bytes of a CPU tensor's storage."""
+    base = state.data_ptr()
+    store = state.untyped_storage()
+    raw = torch.empty(0, dtype=torch.uint8).set_(store)
+    before = raw.clone()
+    off0 = base - store.data_ptr()
+    for o0 in range(desc.outer[0]):
+        for o1 in range(desc.outer[1]):
+            for r in range(R):
+                live = desc.seg_bytes
+                if lengths is not None and desc.step_bytes:
+                    live = min(live, max(0, int(lengths[r])) * desc.step_bytes)
+                seg = off0 + o0 * desc.outer_stride[0] + o1 * desc.outer_stride[1] + r * K * desc.beam_stride
+                for j in range(K):
+                    src, dst = seg + int(parents[r, j]) * desc.beam_stride, seg + j * desc.beam_stride
+                    raw[dst:dst + live] = before[src:src + live]
+
+
+@pytest.mark.parametrize("shape,dim,length_dim,perm", [
+    ((6,), 0, None, None),
+    ((6, 5), 0, 1, None),
+    ((2, 6, 3, 4, 5), 1, 3, None),
+    ((2, 6, 4, 3, 5), 1, 2, None),
+    ((2, 2, 6, 3, 4), 2, 4, None),
+    ((6, 3, 4, 5), 0, 2, (2, 0, 1, 3)),  # beams not outermost in memory
+    ((6, 1, 4), 0, None, None),
+    ((3, 6), 1, None, None),
+])
+def test_description_of_states(shape, dim, length_dim, perm):
+    R, K = 2, 3
+    g = torch.Generator().manual_seed(3)
+    if perm is None:
+        state = torch.randn(shape, generator=g)
+    else:
+        state = torch.randn([shape[i] for i in perm], generator=g).permute([perm.index(i) for i in range(len(perm))])
+        assert state.shape == shape
+        length_dim = None  # positions are not contiguous in this one
+    parents = torch.tensor([[2, 0, 2], [1, 1, 0]])
+    for lengths in ([None] if length_dim is None else [None, torch.tensor([1, 3], dtype=torch.int32)]):
+        s = state.clone(memory_format=torch.preserve_format)
+        assert s.stride() == state.stride()
+        want = s.clone()
+        for r in range(R):
+            for j in range(K):
+                src = state.select(dim, r * K + int(parents[r, j]))
+                dst = want.select(dim, r * K + j)
+                if lengths is None:
+                    dst.copy_(src)
+                else:
+                    dst.narrow(length_dim - 1, 0, int(lengths[r])).copy_(src.narrow(length_dim - 1, 0, int(lengths[r])))
+        desc = _lib.FmmsBeamState()
+        beam._describe(s, dim, length_dim if lengths is not None else None, R, K, desc, lengths is not None)
+        _moved(s, desc, R, K, parents, lengths)
+        assert torch.equal(s, want)
+
+
+def test_description_refuses():
+    desc = _lib.FmmsBeamState()
+    with pytest.raises(ValueError):  # another number of beams
+        beam._describe(torch.zeros(5, 4), 0, None, 2, 3, desc, False)
+    with pytest.raises(ValueError):  # shared memory
+        beam._describe(torch.zeros(1, 4).expand(6, 4), 0, None, 2, 3, desc, False)
+    with pytest.raises(ValueError):  # windows that overlap
+        beam._describe(torch.zeros(20).unfold(0, 5, 3), 0, None, 2, 3, desc, False)
+    with pytest.raises(ValueError):  # positions that are not contiguous
+        beam._describe(torch.zeros(6, 4, 8)[..., ::2], 0, 1, 2, 3, desc, True)
+    with pytest.raises(ValueError):  # three uneven dimensions around the beams
+        beam._describe(torch.zeros(4, 3, 6, 4, 5)[::2, ::2, :, ::2], 2, None, 2, 3, desc, False)

@@ -1,0 +1,247 @@
+"""4-bit products against the dequantised weight in 64 bits.
+
+Tolerance.  Every product of a code (4 bits) with an x in fp16 is exact, and x reaches fp16 exactly unless it lies below
+2^-28 of its row's maximum (then within 2^-39 of that maximum).  What rounds are fp32 additions.  Tensor cores may
+truncate (2^-23 relative to the largest partial sum) and every partial sum is at most A = sum_k scale (q + zero) |x|.  An
+output passes through at most 16 additions inside a product, group / 16 products, cols / group group sums, 16 warps, 8
+CTAs, and 8 further roundings (sums of x, zero point, scales, powers of two): error <= n 2^-23 A with that n.  The
+output type adds half a step: eps / 2 relative.
+"""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def fs():
+    import flashsampling_b200 as fs
+    from flashsampling_b200 import build
+
+    build.build_library()
+    return fs
+
+
+def _dev():
+    return torch.device("cuda", 0)
+
+
+def _weight(fs, rows, cols, group, zeros, seed=0, scale_dtype=torch.bfloat16):
+    g = torch.Generator(device=_dev()).manual_seed(seed)
+    q = torch.randint(0, 16, (rows, cols), generator=g, device=_dev(), dtype=torch.uint8)
+    s = ((torch.rand(rows, cols // group, generator=g, device=_dev()) + 0.5) * 0.01).to(scale_dtype)
+    z = torch.randint(0, 16, (rows, cols // group), generator=g, device=_dev(), dtype=torch.uint8) if zeros else None
+    return fs.Int4Weight.from_rows(q, s, z)
+
+
+def _x(batch, cols, dtype, seed=1):
+    g = torch.Generator(device=_dev()).manual_seed(seed)
+    x = torch.randn(batch, cols, generator=g, device=_dev())
+    x[:, ::97] *= 30
+    return x.to(dtype)
+
+
+def _reference(w, x):
+    """The result in 64 bits and the bound of its computation in 32."""
+    wd = w.dequantize(torch.float64)
+    scale = w.scales.permute(0, 3, 2, 1).reshape(-1, w.scales.shape[1])[:w.rows].double().repeat_interleave(w.group_size, 1)
+    zero = 8.0 if w.zeros is None else w.zeros.permute(0, 3, 2, 1).reshape(-1, w.scales.shape[1])[:w.rows].double().repeat_interleave(w.group_size, 1)
+    xd = x.double().reshape(-1, w.cols)
+    amount = xd.abs() @ (scale.abs() * (w.codes().double() + zero)).T
+    n = 16 + w.group_size // 16 + w.cols // w.group_size + 16 + 8 + 8
+    tiny = xd.abs().amax(1, keepdim=True) * 2.0**-39 * (scale.abs() * 16).sum(1)
+    shape = x.shape[:-1] + (w.rows,)
+    return (xd @ wd.T).view(shape), (n * 2.0**-23 * amount + tiny).view(shape)
+
+
+def _check(y, want, bound):
+    tol = bound + want.abs() * torch.finfo(y.dtype).eps / 2 + torch.finfo(y.dtype).tiny
+    over = (y.double() - want).abs() > tol
+    assert not bool(over.any()), f"{int(over.sum())} of {over.numel()} outputs off, worst {float(((y.double() - want).abs() / tol).max()):.2f} of the bound"
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("rows,cols,batch", [(1, 256, 1), (16, 256, 1), (17, 512, 3), (100, 1024, 8), (250, 768, 9),
+                                              (333, 2048, 16), (64, 4352, 17), (2500, 1280, 32), (75, 512, 70)])
+def test_against_the_dequantised_weight(fs, rows, cols, batch, group, zeros):
+    w = _weight(fs, rows, cols, group, zeros, seed=rows + group)
+    x = _x(batch, cols, torch.bfloat16, seed=cols)
+    want, bound = _reference(w, x)
+    _check(fs.int4_linear(x, w, out_dtype=torch.float32), want, bound)
+    fs.check_status()
+
+
+@pytest.mark.parametrize("cols", [32, 96, 160, 4128])
+def test_half_filled_last_chunk(fs, cols):
+    w = _weight(fs, 130, cols, 32, True, seed=cols)
+    x = _x(5, cols, torch.float16)
+    want, bound = _reference(w, x)
+    _check(fs.int4_linear(x, w, out_dtype=torch.float32), want, bound)
+
+
+@pytest.mark.parametrize("xt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("st", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("ot", [torch.bfloat16, torch.float16, torch.float32, None])
+def test_types(fs, xt, st, ot):
+    w = _weight(fs, 200, 640, 64, True, scale_dtype=st)
+    x = _x(4, 640, xt)
+    y = fs.int4_linear(x, w, out_dtype=ot)
+    assert y.dtype == (ot or xt)
+    _check(y, *_reference(w, x))
+
+
+@pytest.mark.parametrize("rows,cols,batch,group", [
+    (40, 16384, 1, 128),  # few tiles, long rows: a cluster per tile
+    (40, 16384, 16, 128),
+    (9000, 8192, 16, 128),  # x of 16 rows does not fit one CTA
+    (3000, 16384, 30, 64),
+    (500, 28672, 8, 256),
+    (48, 65536, 9, 256),  # falls back to fewer rows per pass
+])
+def test_columns_split_over_a_cluster(fs, rows, cols, batch, group):
+    w = _weight(fs, rows, cols, group, True, seed=rows)
+    x = _x(batch, cols, torch.bfloat16)
+    want, bound = _reference(w, x)
+    _check(fs.int4_linear(x, w, out_dtype=torch.float32), want, bound)
+    fs.check_status()
+
+
+@pytest.mark.parametrize("rows,cols,batch", [(151936, 4096, 1), (32776, 5376, 5), (16032, 8192, 12)])
+def test_heads(fs, rows, cols, batch):
+    w = _weight(fs, rows, cols, 128, True, seed=3)
+    x = _x(batch, cols, torch.bfloat16)
+    y = fs.int4_linear(x, w, out_dtype=torch.float32)
+    at = torch.cat([torch.arange(0, 64), torch.randint(0, rows, (4000,), generator=torch.Generator().manual_seed(0)), torch.arange(rows - 64, rows)])
+    q, at = w.codes(), at.to(_dev())
+    s = w.scales.permute(0, 3, 2, 1).reshape(-1, w.scales.shape[1])[:rows]
+    z = w.zeros.permute(0, 3, 2, 1).reshape(-1, w.scales.shape[1])[:rows]
+    part = fs.Int4Weight.from_rows(q[at].contiguous(), s[at].contiguous(), z[at].contiguous())
+    want, bound = _reference(part, x)
+    _check(y[:, at], want, bound)
+
+
+def test_magnitudes_of_x(fs):
+    """Each row is scaled by itself: rows of 1e-30 and of 1e30 beside each other, and small values beside large ones."""
+    w = _weight(fs, 64, 512, 128, True)
+    x = _x(8, 512, torch.bfloat16)
+    x[1] *= 1e30
+    x[2] *= 1e-30
+    x[3] = 0
+    x[4, 0] = 3e30
+    x[5] = torch.finfo(torch.bfloat16).tiny
+    x[6] = 0
+    x[6, 77] = 1
+    want, bound = _reference(w, x)
+    y = fs.int4_linear(x, w, out_dtype=torch.float32)
+    _check(y, want, bound)
+    assert bool((y[3] == 0).all())
+    h = _x(3, 512, torch.float16)
+    h[0] = torch.finfo(torch.float16).max
+    h[1] = 2.0**-24
+    _check(fs.int4_linear(h, w, out_dtype=torch.float32), *_reference(w, h))
+
+
+def test_rows_that_are_not_finite_stay_alone(fs):
+    w = _weight(fs, 64, 512, 128, False)
+    x = _x(4, 512, torch.bfloat16)
+    clean = fs.int4_linear(x, w, out_dtype=torch.float32)
+    x[1, 5] = float("nan")
+    x[3, 9] = float("inf")
+    y = fs.int4_linear(x, w, out_dtype=torch.float32)
+    assert torch.equal(y[0], clean[0]) and torch.equal(y[2], clean[2])
+    assert not bool(y[1].isfinite().any()) and not bool(y[3].isfinite().any())
+
+
+def test_strided_and_unaligned_x_and_out(fs):
+    w = _weight(fs, 300, 512, 128, True)
+    wide = _x(6, 2 * 512 + 3, torch.bfloat16)
+    for x in (wide[:, 1:513], wide[:, 8:520], wide[::2, 3:515], wide[:, 0:1024:2], wide[:1, 5:517]):
+        _check(fs.int4_linear(x, w, out_dtype=torch.float32), *_reference(w, x))
+    x = _x(6, 512, torch.bfloat16)
+    want, bound = _reference(w, x)
+    buf = torch.full((6, 777), 7.0, device=_dev())
+    y = fs.int4_linear(x, w, out=buf[:, 100:400])
+    assert y.data_ptr() == buf[:, 100:].data_ptr()
+    _check(buf[:, 100:400], want, bound)
+    assert bool((buf[:, :100] == 7).all()) and bool((buf[:, 400:] == 7).all())  # nothing else is written
+
+
+def test_leading_dimensions_and_empty_batch(fs):
+    w = _weight(fs, 100, 256, 64, False)
+    x = _x(6, 256, torch.float16)
+    flat = fs.int4_linear(x, w)
+    assert torch.equal(fs.int4_linear(x.view(2, 3, 256), w), flat.view(2, 3, 100))
+    assert torch.equal(fs.int4_linear(x[2], w), flat[2])
+    assert fs.int4_linear(x[:0], w).shape == (0, 100)
+    out = torch.empty(2, 3, 100, dtype=torch.float16, device=_dev())
+    assert fs.int4_linear(x.view(2, 3, 256), w, out=out) is out and torch.equal(out.view(6, 100), flat)
+
+
+def test_same_bits_every_time_and_in_every_batch(fs):
+    w = _weight(fs, 3333, 4096, 128, True)
+    x = _x(8, 4096, torch.bfloat16)
+    first = fs.int4_linear(x, w, out_dtype=torch.float32)
+    for _ in range(5):
+        assert torch.equal(fs.int4_linear(x, w, out_dtype=torch.float32), first)
+    for b in range(8):
+        assert torch.equal(fs.int4_linear(x[b:b + 1], w, out_dtype=torch.float32)[0], first[b])
+
+
+def test_streams_and_graphs(fs):
+    w = _weight(fs, 2000, 2048, 64, True)
+    xs = [_x(3, 2048, torch.bfloat16, seed=s) for s in range(4)]
+    want = [fs.int4_linear(x, w) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = []
+    for s, x in zip(streams, xs):
+        with torch.cuda.stream(s):
+            got.append([fs.int4_linear(x, w) for _ in range(3)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, e) for ys, e in zip(got, want) for y in ys)
+    static = xs[0].clone()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = fs.int4_linear(static, w)
+        graphs.append((g, y))
+    for x, e in zip(xs, want):
+        static.copy_(x)
+        torch.cuda.synchronize()
+        for (g, _), s in zip(graphs, streams):  # both at once, on streams of their own
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, e) for _, y in graphs)
+    fs.check_status()
+
+
+def test_refusals(fs):
+    w = _weight(fs, 64, 256, 64, False)
+    x = _x(2, 256, torch.bfloat16)
+    with pytest.raises(TypeError):
+        fs.int4_linear(x.float(), w)
+    with pytest.raises(ValueError):
+        fs.int4_linear(x[:, :128], w)
+    with pytest.raises(RuntimeError):
+        fs.int4_linear(x.cpu(), w)
+    with pytest.raises(RuntimeError):
+        fs.int4_linear(x, w.to("cpu"))
+    with pytest.raises(TypeError):
+        fs.int4_linear(x, w, out_dtype=torch.float64)
+    with pytest.raises(ValueError):
+        fs.int4_linear(x, w, out=torch.empty(2, 65, device=_dev()))
+    with pytest.raises(ValueError):
+        fs.int4_linear(x, w, out=torch.empty(64, 2, device=_dev()).T)
+    with pytest.raises(ValueError):
+        fs.int4_linear(x, w, out=torch.empty(2, 64, device=_dev()), out_dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="backward"):
+        fs.int4_linear(x.clone().requires_grad_(), w)
+    with torch.no_grad():
+        fs.int4_linear(x.clone().requires_grad_(), w)
+    big = _weight(fs, 16, 256 * 1024, 256, False)
+    with pytest.raises(fs._lib.FmmsError, match="unsupported"):
+        fs.int4_linear(_x(1, 256 * 1024, torch.bfloat16), big)  # a row of x does not fit eight CTAs

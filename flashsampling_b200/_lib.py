@@ -165,9 +165,10 @@ SIGNATURES = {
             c_void_p, c_void_p, c_int, c_void_p,  # qweight, scales, scale_dtype, zeros
             c_int, c_int, c_int, c_int,  # V, D, group, B
             c_void_p, c_int, c_longlong,  # out, out_dtype, out_stride
-            c_void_p, c_void_p,  # status_dev, stream
+            c_void_p, c_size_t, c_void_p,  # workspace, workspace_bytes, stream
         ],
     ),
+    "fmms_query_int4_workspace": (c_int, [c_int, c_int, c_int, c_int, ctypes.POINTER(c_size_t)]),
     "fmms_query_beam_workspace": (c_int, [c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(c_size_t)]),
     "fmms_beam_step": (
         c_int,
@@ -240,6 +241,12 @@ def query_staging(d: int, b: int, s: int) -> int:
     n = c_size_t(0)
     check(load().fmms_query_staging(d, b, s, ctypes.byref(n)), "fmms_query_staging")
     return int(n.value)
+
+
+def query_int4_workspace(v: int, d: int, group: int, b: int) -> int:
+    nbytes = c_size_t(0)
+    check(load().fmms_query_int4_workspace(v, d, group, b, ctypes.byref(nbytes)), "fmms_query_int4_workspace")
+    return int(nbytes.value)
 
 
 def query_beam_workspace(r: int, k: int, v: int, n: int, dtype: int) -> int:

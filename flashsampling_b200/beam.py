@@ -182,7 +182,7 @@ def reorder_beams(
     """Beam ``j`` of request ``r`` continues beam ``parents[r, j]``: in every state, in place,
     ``state[.., r * beams + j, ..] = state[.., r * beams + parents[r, j], ..]``, all beams at once.
 
-    With ``lengths`` only the first ``lengths[r]`` positions along ``length_dim`` move; what lies behind them stays as it
+    Without ``lengths`` whole beams move.  With ``lengths`` only the first ``lengths[r]`` positions along ``length_dim`` move; what lies behind them stays as it
     is (lengths beyond the dimension count as all of it).  A parent outside ``0..beams-1`` keeps the beam's own state.
     One launch for up to 64 tensors; a beam that keeps its own state costs no traffic.  Up to 64 beams.  States may
     be strided views as long as they do not overlap, themselves or one another."""
@@ -195,8 +195,8 @@ def reorder_beams(
     if K < 1 or K > 64:
         raise ValueError("reorder_beams takes 1 to 64 beams")
     dev = parents.device
-    if (lengths is None) != (length_dim is None):
-        raise ValueError("lengths and length_dim go together")
+    if lengths is not None and length_dim is None:
+        raise ValueError("lengths needs length_dim, the states' dimension of positions")
     if lengths is not None:
         if lengths.shape != (R,) or lengths.dtype not in (torch.int32, torch.int64) or lengths.device != dev:
             raise ValueError(f"lengths must be int32 or int64 [{R}] on {dev}")
@@ -214,7 +214,7 @@ def reorder_beams(
         if s.is_complex() or s.is_sparse or s.is_quantized:
             raise TypeError("states must be plain dense tensors")
         d = dim + s.ndim if dim < 0 else dim
-        ld = None if length_dim is None else (length_dim + s.ndim if length_dim < 0 else length_dim)
+        ld = None if lengths is None else (length_dim + s.ndim if length_dim < 0 else length_dim)
         if not 0 <= d < s.ndim or (ld is not None and not d < ld < s.ndim):
             raise ValueError(f"a state of {s.ndim} dimensions has no beams along {dim}, or no positions behind them along {length_dim}")
         _describe(s, d, ld, R, K, descs[n], lengths is not None)

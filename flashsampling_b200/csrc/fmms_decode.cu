@@ -36,44 +36,50 @@ static int decode_num_sms(int* dev_out, int* sms_out) {
 
 // ---- products with 4-bit weights ----------------------------------------------------------------
 struct Int4Plan {
-  int nt, split, warps, stages, stage_bytes, smem;
-  int xs_off, ring_off, red_off, join_off, bar_off;
+  int nt, warps, phases, units, all_units, smem;
+  int xs_off, xs32_off, ring_off, piece_off;
 };
 
-static int int4_smem(Int4Plan& pl, int cta_chunks, int group) {
-  const int gran = group > 64 ? group / 64 : 1, per_chunk = group < 64 ? 64 / group : 1;
-  pl.stage_bytes = kInt4StepChunks * 512 + kInt4StepChunks * per_chunk / gran * 48;
-  int off = cta_chunks * pl.nt * 1024;
+static int int4_smem(Int4Plan& pl, int group) {
+  int off = pl.units * 2 * pl.nt * 1024;
   pl.xs_off = off;
-  off += (cta_chunks * per_chunk / gran * pl.nt * 32 + 127) / 128 * 128;
+  off += (pl.units * int4_unit_groups(group) * pl.nt * 32 + 127) / 128 * 128;
+  pl.xs32_off = off;
+  if (group > 32) off += pl.units * 4 * pl.nt * 32;
+  pl.piece_off = off;
+  off += pl.warps * 2 * pl.nt * 512;
   pl.ring_off = off;
-  off += pl.warps * pl.stages * pl.stage_bytes;
-  pl.red_off = off;
-  off += 2 * pl.warps * pl.nt * 512;
-  pl.join_off = off;
-  if (pl.split > 1) off += 2 * pl.split * pl.nt * 512;
-  pl.bar_off = off;
-  off += pl.warps * pl.stages * 8;
+  off += pl.warps * kInt4Stages * int4_stage_bytes(group);
   pl.smem = off;
   return off;
 }
 
-// Blocks of eight rows of x per pass: all of x where shared memory holds it (a cluster of up to eight CTAs splits the
-// columns between them), else as many as fit.
-static bool int4_plan(Int4Plan& pl, int V, int D, int B, int group, int num_sms) {
-  const int gran = group > 64 ? group / 64 : 1;
-  const int chunks = (D + kInt4Chunk - 1) / kInt4Chunk, units = chunks / gran, tiles = (V + kInt4Tile - 1) / kInt4Tile;
-  for (pl.nt = B <= 8 ? 1 : B <= 16 ? 2 : 4; pl.nt >= 1; pl.nt >>= 1) {
-    pl.warps = pl.nt == 4 ? 8 : kInt4MaxWarps;
-    for (pl.split = 1; pl.split <= 8 && pl.split <= units; pl.split *= 2) {
-      const int cta_chunks = (units + pl.split - 1) / pl.split * gran;
-      // few tiles: also split while that gives idle SMs work and every warp keeps a fetch of its own
-      if (pl.split < 8 && tiles * pl.split * 2 <= num_sms && cta_chunks >= 2 * pl.warps * kInt4StepChunks) continue;
-      for (pl.stages = kInt4MaxStages; pl.stages >= 2; --pl.stages)
-        if (int4_smem(pl, cta_chunks, group) <= kInt4SmemLimit) return true;
-    }
-  }
-  return false;
+// Blocks of eight rows of x per pass, warps, and the phases x takes.  16 warps hide the products' latency best (head of
+// 151936 x 4096, B = 1: 55.9 us against 57.7 with 8), but their larger buffers leave less room for x: up to 16 rows run
+// with 8 warps where those, and not 16, take all of x at once (the same head, B = 16: 93 us against 110; 262208 x 5376,
+// which takes several phases either way: 250 against 201).  More rows need the registers of 8 warps.
+static int int4_plan(Int4Plan& pl, int D, int B, int group) {
+  pl.all_units = (D + kInt4Unit - 1) / kInt4Unit;
+  pl.nt = B <= 8 ? 1 : B <= 16 ? 2 : 4;
+  auto fits = [&](int warps, int phases) {
+    pl.warps = warps;
+    pl.phases = phases;
+    pl.units = (pl.all_units + phases - 1) / phases;
+    return (phases - 1) * pl.units < pl.all_units &&  // the last phase is not empty
+           int4_smem(pl, group) <= kInt4SmemLimit;
+  };
+  if (pl.nt == 2 && !fits(16, 1) && fits(8, 1)) return kOk;
+  for (int phases = 1; phases <= pl.all_units; ++phases)
+    if (fits(pl.nt == 4 ? 8 : 16, phases)) return kOk;
+  return kErrUnsupported;
+}
+
+static bool int4_group_ok(int group, int D) { return (group == 32 || group == 64 || (group > 0 && group % kInt4Unit == 0)) && D % group == 0; }
+
+static size_t int4_workspace(const Int4Plan& pl, int V, int B) {
+  if (pl.phases == 1) return 0;
+  const size_t tiles = (V + kInt4Tile - 1) / kInt4Tile, blocks = (B + pl.nt * 8 - 1) / (pl.nt * 8);
+  return blocks * (tiles + 1) * pl.nt * 512;
 }
 
 template <int NT, int GR, bool ZP>
@@ -87,25 +93,9 @@ static int int4_launch(const Int4Params& p, const Int4Plan& pl, int dev, int num
     }
     ready[dev].store(true, std::memory_order_release);
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(min(p.tiles, num_sms / pl.split) * pl.split), (unsigned)((p.B + NT * 8 - 1) / (NT * 8)));
-  cfg.blockDim = dim3((unsigned)pl.warps * 32);
-  cfg.dynamicSmemBytes = (size_t)pl.smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  if (pl.split > 1) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)pl.split;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-  }
-  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
-    cudaGetLastError();
-    return kErrCuda;
-  }
-  return kOk;
+  const dim3 grid((unsigned)min(p.tiles, num_sms), (unsigned)((p.B + NT * 8 - 1) / (NT * 8)));
+  kernel<<<grid, pl.warps * 32, pl.smem, stream>>>(p);
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
 
 template <int NT, bool ZP>
@@ -113,8 +103,7 @@ static int int4_launch_group(const Int4Params& p, const Int4Plan& pl, int group,
   switch (group) {
     case 32: return int4_launch<NT, 32, ZP>(p, pl, dev, num_sms, stream);
     case 64: return int4_launch<NT, 64, ZP>(p, pl, dev, num_sms, stream);
-    case 128: return int4_launch<NT, 128, ZP>(p, pl, dev, num_sms, stream);
-    default: return int4_launch<NT, 256, ZP>(p, pl, dev, num_sms, stream);
+    default: return int4_launch<NT, 128, ZP>(p, pl, dev, num_sms, stream);
   }
 }
 
@@ -164,22 +153,34 @@ using namespace fmms;
 
 extern "C" {
 
+int fmms_query_int4_workspace(int V, int D, int group, int B, size_t* bytes) {
+  if (!bytes || V <= 0 || D <= 0 || B <= 0) return FMMS_ERR_BAD_ARG;
+  if (!int4_group_ok(group, D)) return FMMS_ERR_UNSUPPORTED;
+  Int4Plan pl;
+  const int rc = int4_plan(pl, D, B, group);
+  if (rc == kOk) *bytes = int4_workspace(pl, V, B);
+  return rc;
+}
+
 int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void* qweight, const void* scales, int scale_dtype,
                      const void* zeros, int V, int D, int group, int B, void* out, int out_dtype, long long out_stride,
-                     int* status_dev, void* stream) {
+                     void* workspace, size_t workspace_bytes, void* stream) {
   if (!x || !qweight || !scales || !out || V <= 0 || D <= 0 || B <= 0) return FMMS_ERR_BAD_ARG;
   if ((x_dtype != FMMS_BF16 && x_dtype != FMMS_F16) || (scale_dtype != FMMS_BF16 && scale_dtype != FMMS_F16) ||
       out_dtype < FMMS_BF16 || out_dtype > FMMS_F32)
     return FMMS_ERR_BAD_ARG;
   if (x_stride < D || out_stride < V) return FMMS_ERR_BAD_ARG;
-  if ((group != 32 && group != 64 && group != 128 && group != 256) || D % group != 0) return FMMS_ERR_UNSUPPORTED;
+  if (!int4_group_ok(group, D)) return FMMS_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(qweight) | reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(zeros)) & 15)
     return FMMS_ERR_UNSUPPORTED;
-  int dev = 0, num_sms = 0;
-  const int rc = decode_num_sms(&dev, &num_sms);
-  if (rc != kOk) return rc;
   Int4Plan pl;
-  if (!int4_plan(pl, V, D, B, group, num_sms)) return FMMS_ERR_UNSUPPORTED;
+  int rc = int4_plan(pl, D, B, group);
+  if (rc != kOk) return rc;
+  const size_t need = int4_workspace(pl, V, B);
+  if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need)) return FMMS_ERR_WORKSPACE;
+  int dev = 0, num_sms = 0;
+  rc = decode_num_sms(&dev, &num_sms);
+  if (rc != kOk) return rc;
   Int4Params p = {};
   p.x = x;
   p.x_stride = x_stride;
@@ -197,16 +198,18 @@ int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void*
   p.x_bf16 = x_dtype == FMMS_BF16;
   p.s_bf16 = scale_dtype == FMMS_BF16;
   p.out_kind = out_dtype - FMMS_BF16;
-  p.x_vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && x_stride % 8 == 0;
-  p.split = pl.split;
-  p.stages = pl.stages;
-  p.stage_bytes = pl.stage_bytes;
+  p.x_pairs = (reinterpret_cast<uintptr_t>(x) & 3) == 0 && x_stride % 2 == 0;
+  for (p.log_rows = 0; (1 << p.log_rows) < min(B, pl.nt * 8); ++p.log_rows) {
+  }
+  p.xs32_off = pl.xs32_off;
+  p.partial = reinterpret_cast<float*>(workspace);
+  p.group_units = group > kInt4Unit ? group / kInt4Unit : 1;
+  p.phases = pl.phases;
+  p.units = pl.units;
+  p.all_units = pl.all_units;
   p.xs_off = pl.xs_off;
   p.ring_off = pl.ring_off;
-  p.red_off = pl.red_off;
-  p.join_off = pl.join_off;
-  p.bar_off = pl.bar_off;
-  p.status_dev = status_dev;
+  p.piece_off = pl.piece_off;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return zeros ? int4_launch_rows<true>(p, pl, group, dev, num_sms, s) : int4_launch_rows<false>(p, pl, group, dev, num_sms, s);
 }

@@ -15,12 +15,16 @@
 //   down to 2^-28 of the row's maximum keep all their bits, smaller ones are rounded to 2^-39 of that maximum, which is
 //   below the rounding of the fp32 sums.
 //
-// Work split.  A tile is 16 weight rows over all columns, contiguous in memory.  A persistent CTA (or, for long rows
-// and few tiles, a cluster of them) takes one tile at a time; its warps split the columns, so that the hidden states a
-// warp multiplies with stay at fixed places of shared memory, laid out in operand order.  Every warp streams its own
-// part of the tile through a private ring of bulk copies (one lane issues, the warp waits on the mbarrier; no other warp
-// is involved until the tile's sums are joined through shared memory).  Clusters join their sums in the first CTA's
-// shared memory.  No atomics, one order of additions: results do not depend on timing, nor a row on its batch.
+// Work split.  Tiles of 16 rows are dealt to the CTAs, one per SM, in contiguous ranges; the warps of a CTA share its
+// range in equal parts that begin and end anywhere in a pair of tiles (two at a time share the operand loads of x).  A
+// warp's part is contiguous in memory and it streams it through a ring of asynchronous copies of its own: between the
+// load of x and the end of the stream no warp waits for another.  A pair that several warps have a part of is joined at
+// the end in the order of the columns: the first keeps its sums in registers, the others leave theirs in shared memory.
+// (Bulk copies cost here: about 75 cycles of issue each from one producer warp, and with 32 to 1024 bytes to a copy
+// there are four to six per 2 KiB; per-lane copies of 16 bytes need one instruction per 512.)
+// x lies in shared memory in operand order.  Where it does not fit, the columns are taken in phases, and finished sums
+// of a phase wait in global memory for the thread that wrote them.
+// No atomics, one order of additions: results do not depend on timing, nor a row on the rest of its batch.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -29,11 +33,12 @@
 
 namespace fmms {
 
-constexpr int kInt4Tile = 16;        // weight rows of a tile
-constexpr int kInt4Chunk = 64;       // columns of a chunk: 512 bytes of a tile
-constexpr int kInt4StepChunks = 4;   // chunks a warp fetches at a time
-constexpr int kInt4MaxWarps = 16;
-constexpr int kInt4MaxStages = 8;
+constexpr int kInt4Tile = 16;    // weight rows of a tile
+constexpr int kInt4Chunk = 64;   // columns of a chunk: 512 bytes of a tile
+constexpr int kInt4Stages = 3;   // units in a warp's ring (4 measured the same with 8 warps and worse with 16)
+constexpr int kInt4Unit = 128;   // columns a warp fetches at a time; larger groups apply their scale to several units
+__host__ __device__ constexpr int int4_unit_groups(int group) { return group < kInt4Unit ? kInt4Unit / group : 1; }
+__host__ __device__ constexpr int int4_stage_bytes(int group) { return 2 * (2 * 512 + int4_unit_groups(group) * 48); }
 
 struct Int4Params {
   const void* x;
@@ -43,55 +48,57 @@ struct Int4Params {
   const uint8_t* zeros;        // [tiles][groups][8][2], or null: 8
   void* out;
   long long out_stride;        // elements between rows of out
+  float* partial;              // [row blocks][tiles][NT * 128], several phases only
   int V, D, B;
   int tiles, chunks, groups;
   int x_bf16, s_bf16, out_kind;  // out_kind: 0 bf16, 1 fp16, 2 fp32
-  int x_vec;                   // rows of x start on 16-byte boundaries
-  int split;                   // CTAs of a cluster, each with its share of the columns
-  int stages, stage_bytes;
-  int xs_off, ring_off, red_off, join_off, bar_off;  // shared memory
-  int* status_dev;
+  int x_pairs;                 // rows of x start on 4-byte boundaries
+  int log_rows;                // rows of x in a pass, rounded up to a power of two
+  int group_units;             // units of a group (1 for groups of up to 128 columns)
+  int phases, units, all_units;  // units of a phase (the last one may have fewer) and of a row
+  int xs_off, xs32_off, ring_off, piece_off;  // shared memory
 };
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t pol) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
-          smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(pol)
-      : "memory");
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 
+// c = A B + c0 for a 16 x 16 A and a 16 x 8 B
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                                          uint32_t b1, float c0, float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+
+// two fp32 additions, and two multiplications by s with additions, in one instruction each
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+  const float2 r = __fadd2_rn(make_float2(x, y), make_float2(a, b));
+  x = r.x;
+  y = r.y;
+}
+__device__ __forceinline__ void fma2(float& x, float& y, float s, float a, float b) {
+  const float2 r = __ffma2_rn(make_float2(s, s), make_float2(a, b), make_float2(x, y));
+  x = r.x;
+  y = r.y;
 }
 
 __device__ __forceinline__ float half_bits_to_float(uint32_t bits16, bool bf16) {
   return bf16 ? __uint_as_float(bits16 << 16) : __half2float(__ushort_as_half((unsigned short)bits16));
 }
 
-// Eight consecutive elements of a row of x as fp32 (k is a multiple of 8, the row length a multiple of 32).
-__device__ __forceinline__ void int4_load_x8(const Int4Params& p, int b, int k, float (&v)[8]) {
+// Columns k, k + 1 and the three pairs 8, 16 and 24 columns on, of a row of x (k is even).
+__device__ __forceinline__ uint4 int4_load_x(const Int4Params& p, int b, int k) {
   const uint16_t* src = reinterpret_cast<const uint16_t*>(p.x) + (size_t)b * p.x_stride + k;
   uint32_t w[4];
-  if (p.x_vec) {
-    const uint4 u = *reinterpret_cast<const uint4*>(src);
-    w[0] = u.x;
-    w[1] = u.y;
-    w[2] = u.z;
-    w[3] = u.w;
-  } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)src[2 * i] | ((uint32_t)src[2 * i + 1] << 16);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = half_bits_to_float(w[i] & 0xffffu, p.x_bf16);
-    v[2 * i + 1] = half_bits_to_float(w[i] >> 16, p.x_bf16);
-  }
+  for (int i = 0; i < 4; ++i)
+    w[i] = p.x_pairs ? *reinterpret_cast<const uint32_t*>(src + 8 * i) : (uint32_t)src[8 * i] | ((uint32_t)src[8 * i + 1] << 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 __device__ __forceinline__ void int4_store(const Int4Params& p, int b, int v, float y) {
@@ -104,245 +111,367 @@ __device__ __forceinline__ void int4_store(const Int4Params& p, int b, int v, fl
     reinterpret_cast<float*>(p.out)[at] = y;
 }
 
-// NT: blocks of eight rows of x; GR: columns of a group; ZP: zero points given.
+// NT: blocks of eight rows of x; GR: columns of a group, at most 128; ZP: zero points given.
 template <int NT, int GR, bool ZP>
-__global__ void __launch_bounds__(kInt4MaxWarps * 32, 1) int4_linear_kernel(const Int4Params p) {
+__global__ void __launch_bounds__(NT == 4 ? 256 : 512, 1) int4_linear_kernel(const Int4Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int kGran = GR > kInt4Chunk ? GR / kInt4Chunk : 1;   // chunks of a group
-  constexpr int kSteps = GR / 16;                                // products of a group
-  constexpr int kPerChunk = GR < kInt4Chunk ? kInt4Chunk / GR : 1;  // groups of a chunk
-  constexpr int kOut = NT * 128;                                 // values of a tile
-  __shared__ unsigned int row_max[NT * 8];
-  __shared__ int abort_word;
+  constexpr int kChunks = kInt4Unit / kInt4Chunk, kGroups = int4_unit_groups(GR);  // of a unit
+  constexpr int kStage = int4_stage_bytes(GR), S = kInt4Stages;
+  constexpr int kScaleOff = 2 * kChunks * 512, kZeroOff = kScaleOff + 2 * kGroups * 32;
+  constexpr int kScaleCopy = kGroups == 4 ? 8 : 4;                    // bytes a lane copies of the scales
+  constexpr int kScaleLanes = kGroups * 32 / kScaleCopy;              // lanes of one tile
+  constexpr int kZeroLanes = kGroups * 4;
+  __shared__ unsigned int row_max[NT * 8], warp_max[16 * NT * 8];
+  __shared__ int part[18];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, W = blockDim.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int rank = (int)blockIdx.x % p.split, first_tile = (int)blockIdx.x / p.split, tile_step = (int)gridDim.x / p.split;
   const int b0 = blockIdx.y * NT * 8, nb = min(NT * 8, p.B - b0);
 
   uint4* xfrag = reinterpret_cast<uint4*>(smem);
-  float* xs = reinterpret_cast<float*>(smem + p.xs_off);
-  uint8_t* ring = smem + p.ring_off + (size_t)warp * p.stages * p.stage_bytes;
-  float* red = reinterpret_cast<float*>(smem + p.red_off);
-  float* join = reinterpret_cast<float*>(smem + p.join_off);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.bar_off) + warp * p.stages;
-  volatile int* abort_flag = &abort_word;
+  float* xs = reinterpret_cast<float*>(smem + p.xs_off);      // [groups of a phase][NT * 8]
+  float* xs32 = reinterpret_cast<float*>(smem + p.xs32_off);  // the same for 32 columns each (groups of 32: xs)
+  float* pieces = reinterpret_cast<float*>(smem + p.piece_off);  // [warps][2 * NT * 4][32]
+  const uint8_t* ring = smem + p.ring_off + warp * (S * kStage);
+  const uint32_t ring_at = smem_u32(ring);
 
-  // columns of this CTA and of this warp, in units of whole groups (whole chunks for groups below 64)
-  const int units = p.chunks / kGran;
-  const int u_cta = (int)((long long)units * rank / p.split), u_end = (int)((long long)units * (rank + 1) / p.split);
-  const int c_cta = u_cta * kGran, cta_units = u_end - u_cta;
-  const int c_begin = (u_cta + cta_units * warp / W) * kGran, c_end = (u_cta + cta_units * (warp + 1) / W) * kGran;
-  const int nsteps = (c_end - c_begin + kInt4StepChunks - 1) / kInt4StepChunks;
-
-  if (lane == 0)
-    for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1);
-  if (tid == 0) abort_word = 0;
-  for (int i = tid; i < NT * 8; i += blockDim.x) row_max[i] = 0u;
-  fence_mbar_init();
+  // this CTA's tiles in pairs, and the warps' parts of them; position = pair * units + unit
+  const int t_begin = (int)((unsigned long long)p.tiles * blockIdx.x / gridDim.x);
+  const int t_end = (int)((unsigned long long)p.tiles * (blockIdx.x + 1) / gridDim.x);
+  const int pairs = (t_end - t_begin + 1) / 2;
+  if (tid <= W) part[tid] = (int)((long long)pairs * p.units * tid / W);
   __syncthreads();
-  if (p.split > 1) {  // every CTA of the cluster runs before one of them writes into the first one's shared memory
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  }
-
-  // the ring: the warp's steps of all its tiles, one after the other
-  int issue_tile = first_tile, issue_step = 0, issued = 0;
-  const uint64_t pol = policy_evict_first();
-  auto issue = [&](int slot) {
-    if (issue_tile >= p.tiles || nsteps == 0) return;
-    const int c = c_begin + issue_step * kInt4StepChunks, n = min(kInt4StepChunks, c_end - c);
-    const int gr = c * kPerChunk / kGran;
-    const int ng = min(max(n / kGran, 1) * kPerChunk, p.groups - gr);
-    uint8_t* dst = ring + (size_t)slot * p.stage_bytes;
-    const uint32_t qb = n * 512, sb = ng * 32, zb = ZP ? ng * 16 : 0;
-    mbar_arrive_expect_tx(&full[slot], qb + sb + zb);
-    bulk_load(dst, p.q + ((size_t)issue_tile * p.chunks + c) * 512, qb, &full[slot], pol);
-    constexpr int kMaxGroups = kInt4StepChunks * kPerChunk / kGran;
-    bulk_load(dst + kInt4StepChunks * 512, p.scales + ((size_t)issue_tile * p.groups + gr) * 16, sb, &full[slot], pol);
-    if constexpr (ZP)
-      bulk_load(dst + kInt4StepChunks * 512 + kMaxGroups * 32, p.zeros + ((size_t)issue_tile * p.groups + gr) * 16, zb,
-                &full[slot], pol);
-    ++issued;
-    if (++issue_step == nsteps) {
-      issue_step = 0;
-      issue_tile += tile_step;
-    }
+  const int begin = part[warp], end = part[warp + 1];
+  const int p_first = begin / p.units, p_last = (end - 1) / p.units;
+  // the units of pair `pr` in `phase` that belong to this warp: from lo to before hi
+  auto unit_range = [&](int phase, int pr, int& lo, int& hi) {
+    lo = max(begin - pr * p.units, 0);
+    hi = min(min(end - pr * p.units, p.units), p.all_units - phase * p.units);
   };
-  if (lane == 0)
-    for (int i = 0; i < p.stages; ++i) issue(i);
 
-  // x: maximum of each row, then fp16 operands in the order the products read them, and the sums over the groups
-  const int k_begin = c_cta * kInt4Chunk, k_end = min(p.D, (u_end * kGran) * kInt4Chunk);
-  const int segs = (k_end - k_begin + 255) / 256;
-  for (int u = warp; u < nb * segs; u += W) {
-    const int b = u / segs, k = k_begin + (u - b * segs) * 256 + lane * 8;
-    unsigned int m = 0u;
-    if (k < k_end) {
-      float v[8];
-      int4_load_x8(p, b0 + b, k, v);
+  // the ring: one unit of both tiles of a pair at a time, one group of copies each (an empty one behind the end)
+  int f_phase = 0, f_pr = p_first, f_unit = 0, f_left = 0, f_slot = 0, f_in_group = 0;
+  const uint8_t *f_q = p.q, *f_s = nullptr, *f_z = nullptr;
+  long long f_pitch = 0;
+  auto seek = [&] {  // (f_phase, f_pr) or the next pair behind it that this warp has units of
+    for (; f_phase < p.phases; ++f_phase, f_pr = p_first)
+      for (; f_pr <= p_last; ++f_pr) {
+        int lo, hi;
+        unit_range(f_phase, f_pr, lo, hi);
+        if (lo >= hi) continue;
+        f_left = hi - lo;
+        f_unit = f_phase * p.units + lo;
+        const int tile = t_begin + f_pr * 2;
+        const int two = tile + 1 < t_end ? 1 : 0;  // the range may end with a single tile: it is fetched twice
+        f_pitch = two ? (long long)p.chunks * 512 : 0;
+        f_q = p.q + ((long long)tile * p.chunks + f_unit * kChunks) * 512 + lane * 16;
+        const int sm = lane / kScaleLanes, zm = lane / kZeroLanes;
+        const int gr = GR < kInt4Unit ? f_unit * kGroups : f_unit / p.group_units;
+        if (GR == kInt4Unit) f_in_group = f_unit - gr * p.group_units;
+        f_s = reinterpret_cast<const uint8_t*>(p.scales) + ((long long)(tile + (sm & two)) * p.groups + gr) * 32 +
+              (lane % kScaleLanes) * kScaleCopy;
+        if constexpr (ZP)
+          f_z = p.zeros + ((long long)(tile + (zm & two)) * p.groups + gr) * 16 + (lane % kZeroLanes) * 4;
+        return;
+      }
+  };
+  auto fetch = [&] {
+    if (f_left > 0) {
+      const uint32_t dst = ring_at + f_slot * kStage;
+      // a row may end within its last unit: chunks and groups that are not there are not read
+      const int chunks = GR < kInt4Unit ? p.chunks - f_unit * kChunks : kChunks;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+          if (c < chunks) copy_async<16>(dst + (m * kChunks + c) * 512 + lane * 16, f_q + (m ? f_pitch : 0) + c * 512);
+      const int left = GR < kInt4Unit ? p.groups - f_unit * kGroups : kGroups;
+      if (lane < 2 * kScaleLanes && (GR == kInt4Unit || (lane % kScaleLanes) * kScaleCopy < left * 32))
+        copy_async<kScaleCopy>(dst + kScaleOff + lane * kScaleCopy, f_s);
+      if constexpr (ZP)
+        if (lane < 2 * kZeroLanes && (GR == kInt4Unit || (lane % kZeroLanes) * 4 < left * 16)) copy_async<4>(dst + kZeroOff + lane * 4, f_z);
+      f_q += kChunks * 512;
+      if (GR < kInt4Unit || ++f_in_group == p.group_units) {
+        f_in_group = 0;
+        f_s += kGroups * 32;
+        if constexpr (ZP) f_z += kGroups * 16;
+      }
+      ++f_unit;
+      if (++f_slot == S) f_slot = 0;
+      if (--f_left == 0) {
+        ++f_pr;
+        seek();
+      }
     }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) atomicMax(&row_max[b], m);
-  }
-  __syncthreads();
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (begin < end) seek();
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) fetch();
+
+  auto pow2 = [](int e) { return __uint_as_float((uint32_t)(e + 127) << 23); };
   // exponent of the power of two that puts the row's maximum into [2^14, 2^15); clamped to what fp32 can hold
   auto row_exponent = [&](int b) {
     const int e = (int)(row_max[b] >> 23) - 127;
     return row_max[b] == 0u ? 0 : min(14 - e, 120);
   };
-  auto pow2 = [](int e) { return __uint_as_float((uint32_t)(e + 127) << 23); };
-  for (int u = warp; u < nb * segs; u += W) {
-    const int b = u / segs, k = k_begin + (u - b * segs) * 256 + lane * 8;
-    float s = 0.f;
-    if (k < k_end) {
-      const float up = pow2(row_exponent(b));
-      float v[8];
-      int4_load_x8(p, b0 + b, k, v);
-      const int c = (k - k_begin) / kInt4Chunk, step = (k & 63) >> 4, half = (k & 15) >> 3;
-      uint32_t* dst = reinterpret_cast<uint32_t*>(xfrag + ((c * 2 + (step >> 1)) * NT + (b >> 3)) * 32 + (b & 7) * 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __half2 h = __floats2half2_rn(v[2 * i] * up, v[2 * i + 1] * up);
-        dst[i * 4 + (step & 1) * 2 + half] = *reinterpret_cast<const uint32_t*>(&h);
-        s += __low2float(h) + __high2float(h);
-      }
-    }
-#pragma unroll
-    for (int off = 1; off < GR / 8; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    if (k < k_end && (lane & (GR / 8 - 1)) == 0)
-      xs[((k - k_begin) / GR) * (NT * 8) + b] = s * (ZP ? -0x1p-24f : -0x1p-21f);  // in units of the operands; times 8
-  }
-  __syncthreads();
 
-  const int gr_cta = c_cta * kPerChunk / kGran;  // first group of the CTA
-  int slot = 0, parity = 0, buf = 0, consumed = 0;
-  int joined_tile = -1;  // clusters: the tile whose sums are on their way to the first CTA
-
-  auto finish_join = [&](int tile, int jbuf) {  // first CTA of a cluster: add the shares in rank order, write the tile
-    for (int j = tid; j < kOut; j += blockDim.x) {
-      float y = 0.f;
-      for (int r = 0; r < p.split; ++r) y += join[(jbuf * p.split + r) * kOut + j];
-      const int i = j >> 5, l = j & 31;
-      const int n = (i >> 2) * 8 + (l & 3) * 2 + (i & 1), v = tile * kInt4Tile + (l >> 2) + ((i & 2) ? 8 : 0);
-      if (n < nb && v < p.V) int4_store(p, b0 + n, v, y);
-    }
+  float tot[2][NT][4];
+  auto clear = [&] {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) tot[m][nt][j] = 0.f;
   };
-
-  for (int tile = first_tile; tile < p.tiles; tile += tile_step) {
-    float tot[NT][4];
+  auto write_out = [&](int pr) {
+    const int tile = t_begin + pr * 2;
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int m = 0; m < 2; ++m)
+      if (tile + m < t_end)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) tot[i][j] = 0.f;
-    for (int st = 0; st < nsteps; ++st) {
-      mbar_wait(&full[slot], (uint32_t)parity, abort_flag, p.status_dev);
-      const int c = c_begin + st * kInt4StepChunks, n = min(kInt4StepChunks, c_end - c);
-      const uint8_t* src = ring + (size_t)slot * p.stage_bytes;
-      const uint4* qsrc = reinterpret_cast<const uint4*>(src) + lane;
-      const uint32_t* ssrc = reinterpret_cast<const uint32_t*>(src + kInt4StepChunks * 512) + g;
-      const uint16_t* zsrc = reinterpret_cast<const uint16_t*>(src + kInt4StepChunks * 512 + kInt4StepChunks * kPerChunk / kGran * 32) + g;
-      const int gr0 = c * kPerChunk / kGran;
-      for (int cu = 0; cu < n; cu += kGran) {
-        float acc[NT][4];
-#pragma unroll
-        for (int cc = 0; cc < kGran; ++cc) {
-          const uint4 qv = qsrc[(cu + cc) * 32];
-          const uint32_t qw[4] = {qv.x, qv.y, qv.z, qv.w};
-          uint4 xv[NT];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int step = cc * 4 + j;               // product within the unit
-            const int gi = cu * kPerChunk / kGran + step / kSteps;  // group within the fetched step
-            if (step % kSteps == 0) {
-              float z0 = 1.f, z1 = 16.f;
-              if constexpr (ZP) {
-                const uint32_t z = zsrc[gi * 8];
-                z0 = (float)(z & 0xffu);
-                z1 = (float)(z >> 8) * 16.f;
+            const int n = nt * 8 + t * 2 + (j & 1), v = (tile + m) * kInt4Tile + g + ((j & 2) ? 8 : 0);
+            if (n < nb && v < p.V) int4_store(p, b0 + n, v, tot[m][nt][j]);
+          }
+  };
+  int slot = 0;
+
+  for (int phase = 0; phase < p.phases; ++phase) {
+    // x: maximum of each row, then fp16 operands in the order the products read them, and the sums over the groups.
+    // A thread has one row and one t, and 8 of every 32 columns: the 16 bytes of one lane's operands.  Its first loads stay
+    // in registers from the maximum to the conversion.
+    const int k_begin = phase * p.units * kInt4Unit;
+    const int blocks = min(p.units, p.all_units - phase * p.units) * (kInt4Unit / 32);  // of 32 columns; zero from p.D on
+    const int stride = (W * 8) >> p.log_rows, first_block = (tid >> 2) >> p.log_rows;
+    const int row = (tid >> 2) & ((1 << p.log_rows) - 1);
+    constexpr int kAhead = 4;  // loads in flight
+    auto load_blocks = [&](int from, uint4 (&raw)[kAhead]) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int blk = from + i * stride;
+        raw[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < nb && blk < blocks && k_begin + blk * 32 < p.D) raw[i] = int4_load_x(p, b0 + row, k_begin + blk * 32 + t * 2);
+      }
+    };
+    int exponent = 0;
+    if (p.x_bf16) {  // fp16 goes in as it is
+      uint32_t m = 0u;  // magnitudes of bf16 compare like integers
+#pragma unroll 1
+      for (int from = first_block; from < blocks; from += kAhead * stride) {
+        uint4 raw[kAhead];
+        load_blocks(from, raw);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+          m = __vmaxu2(m, __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu), __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu)));
+      }
+      m = max(m & 0xffffu, m >> 16);
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1)  // lanes of the same row
+        if (off < 4 || off >= (4 << p.log_rows)) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
+      if (lane < (4 << p.log_rows) && t == 0 && row < nb) warp_max[warp * (NT * 8) + row] = m << 16;
+      __syncthreads();  // also: the phase before has been read
+      if (tid < nb) {
+        m = 0u;
+        // warps hold max(1, rows / 8) rows each: those of this one come round every so many warps
+        const int every = p.log_rows > 3 ? 1 << (p.log_rows - 3) : 1;
+        for (int w = (tid >> 3) & (every - 1); w < W; w += every) m = max(m, warp_max[w * (NT * 8) + tid]);
+        row_max[tid] = m;
+      }
+      __syncthreads();
+      if (row < nb) exponent = row_exponent(row);
+    } else {
+      __syncthreads();
+    }
+    const float up = pow2(exponent);
+#pragma unroll 1
+    for (int from = first_block; from < blocks; from += kAhead * stride) {
+      uint4 raw[kAhead];
+      load_blocks(from, raw);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int blk = from + i * stride;
+        uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (p.x_bf16) {
+            const __half2 h = __floats2half2_rn(__uint_as_float(w[j] << 16) * up, __uint_as_float(w[j] & 0xffff0000u) * up);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+          s += f.x + f.y;
+        }
+        s += __shfl_xor_sync(0xfu << (lane & 28), s, 1);  // the four lanes of a row and block run together
+        s += __shfl_xor_sync(0xfu << (lane & 28), s, 2);
+        if (row < nb && blk < blocks) {
+          xfrag[(blk * NT + (row >> 3)) * 32 + (row & 7) * 4 + t] = make_uint4(w[0], w[1], w[2], w[3]);
+          // in units of the operands; without zero points times 8
+          if (t == 0) (GR == 32 ? xs : xs32)[blk * (NT * 8) + row] = s * (ZP ? -0x1p-24f : -0x1p-21f);
+        }
+      }
+    }
+    __syncthreads();
+    if constexpr (GR > 32) {
+      for (int i = tid; i < blocks / (GR / 32) * (NT * 8); i += W * 32) {
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < GR / 32; ++j) s += xs32[(i / (NT * 8) * (GR / 32) + j) * (NT * 8) + i % (NT * 8)];
+        xs[i] = s;
+      }
+      __syncthreads();
+    }
+
+    float down[NT][2];  // from the units of the sums to the result
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int n = nt * 8 + t * 2 + i;
+        down[nt][i] = n < nb ? (p.x_bf16 ? pow2(-row_exponent(n)) : 1.f) : 0.f;
+      }
+
+    clear();
+    for (int pr = p_first; pr <= p_last && begin < end; ++pr) {
+      int u, hi;
+      unit_range(phase, pr, u, hi);
+      if (u >= hi) continue;
+      const uint4* xp = xfrag + u * (kChunks * 2 * NT * 32) + lane;
+      const float* xsp = xs + u * (kGroups * NT * 8) + t * 2;
+      for (; u < hi; ++u) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+        __syncwarp();  // scales and zeros were copied by other lanes; and everybody is done with the slot before this one
+        fetch();
+        const uint8_t* src = ring + slot * kStage;
+        const uint4* qsrc = reinterpret_cast<const uint4*>(src) + lane;
+        const uint32_t* ssrc = reinterpret_cast<const uint32_t*>(src + kScaleOff) + g;
+        const uint16_t* zsrc = reinterpret_cast<const uint16_t*>(src + kZeroOff) + g;
+        float acc[2][NT][4];
+#pragma unroll
+        for (int cc = 0; cc < kChunks; ++cc) {
+          uint32_t qw[2][4];
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const uint4 qv = qsrc[(m * kChunks + cc) * 32];
+            qw[m][0] = qv.x;
+            qw[m][1] = qv.y;
+            qw[m][2] = qv.z;
+            qw[m][3] = qv.w;
+          }
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) {  // 32 columns: two products
+            constexpr int kPairs = GR / 32;  // of a group
+            const int gi = (cc * 2 + jj) / kPairs;  // group within the unit
+            const bool first = (cc * 2 + jj) % kPairs == 0, last = (cc * 2 + jj) % kPairs == kPairs - 1;
+            uint4 xv[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) xv[nt] = xp[((cc * 2 + jj) * NT + nt) * 32];
+            // Two products to a chain, chains joined by rounded additions: the tensor cores cut sums off.  All first
+            // products, then all second ones: 2 NT chains in flight.
+            float c[2][NT][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {
+                const uint32_t w = qw[m][jj * 2 + h], w8 = w >> 8;
+                const uint32_t a0 = w & 0x000f000fu, a1 = w & 0x00f000f0u, a2 = w8 & 0x000f000fu, a3 = w8 & 0x00f000f0u;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  if (h == 0)
+                    mma_16816(c[m][nt], a0, a1, a2, a3, xv[nt].x, xv[nt].y, 0.f, 0.f, 0.f, 0.f);
+                  else
+                    mma_16816(c[m][nt], a0, a1, a2, a3, xv[nt].z, xv[nt].w, c[m][nt][0], c[m][nt][1], c[m][nt][2], c[m][nt][3]);
+                }
               }
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                const float2 xsum = *reinterpret_cast<const float2*>(xs + (gr0 + gi - gr_cta) * (NT * 8) + nt * 8 + t * 2);
-                acc[nt][0] = z0 * xsum.x;
-                acc[nt][1] = z0 * xsum.y;
-                acc[nt][2] = z1 * xsum.x;
-                acc[nt][3] = z1 * xsum.y;
+            for (int m = 0; m < 2; ++m) {
+              if (first) {
+                float z0 = 1.f, z1 = 16.f;
+                if constexpr (ZP) {
+                  const uint32_t z = zsrc[(m * kGroups + gi) * 8];
+                  z0 = (float)(z & 0xffu);
+                  z1 = (float)(z >> 8) * 16.f;
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  const float2 xsum = *reinterpret_cast<const float2*>(xsp + gi * (NT * 8) + nt * 8);
+                  acc[m][nt][0] = c[m][nt][0];
+                  acc[m][nt][1] = c[m][nt][1];
+                  acc[m][nt][2] = c[m][nt][2];
+                  acc[m][nt][3] = c[m][nt][3];
+                  fma2(acc[m][nt][0], acc[m][nt][1], z0, xsum.x, xsum.y);
+                  fma2(acc[m][nt][2], acc[m][nt][3], z1, xsum.x, xsum.y);
+                }
+              } else {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  add2(acc[m][nt][0], acc[m][nt][1], c[m][nt][0], c[m][nt][1]);
+                  add2(acc[m][nt][2], acc[m][nt][3], c[m][nt][2], c[m][nt][3]);
+                }
               }
-            }
-            const uint32_t w = qw[j], w8 = w >> 8;
-            const uint32_t a0 = w & 0x000f000fu, a1 = w & 0x00f000f0u, a2 = w8 & 0x000f000fu, a3 = w8 & 0x00f000f0u;
+              if (last && (GR == kInt4Unit || (phase * p.units + u) * kGroups + gi < p.groups)) {
+                const uint32_t s2 = ssrc[(m * kGroups + gi) * 8];
+                const float s0 = half_bits_to_float(s2 & 0xffffu, p.s_bf16);
+                const float s1 = half_bits_to_float(s2 >> 16, p.s_bf16) * 0.0625f;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if ((j & 1) == 0) xv[nt] = xfrag[(((c - c_cta + cu + cc) * 2 + (j >> 1)) * NT + nt) * 32 + lane];
-              if ((j & 1) == 0)
-                mma_16816(acc[nt], a0, a1, a2, a3, xv[nt].x, xv[nt].y);
-              else
-                mma_16816(acc[nt], a0, a1, a2, a3, xv[nt].z, xv[nt].w);
-            }
-            if ((step + 1) % kSteps == 0 && (GR > 32 || gr0 + gi < p.groups)) {
-              const uint32_t s2 = ssrc[gi * 8];
-              const float s0 = half_bits_to_float(s2 & 0xffffu, p.s_bf16), s1 = half_bits_to_float(s2 >> 16, p.s_bf16) * 0.0625f;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                tot[nt][0] = fmaf(s0, acc[nt][0], tot[nt][0]);
-                tot[nt][1] = fmaf(s0, acc[nt][1], tot[nt][1]);
-                tot[nt][2] = fmaf(s1, acc[nt][2], tot[nt][2]);
-                tot[nt][3] = fmaf(s1, acc[nt][3], tot[nt][3]);
+                for (int nt = 0; nt < NT; ++nt) {
+                  fma2(tot[m][nt][0], tot[m][nt][1], s0, acc[m][nt][0], acc[m][nt][1]);
+                  fma2(tot[m][nt][2], tot[m][nt][3], s1, acc[m][nt][2], acc[m][nt][3]);
+                }
               }
             }
           }
         }
+        xp += kChunks * 2 * NT * 32;
+        xsp += kGroups * NT * 8;
+        if (++slot == S) slot = 0;
       }
-      __syncwarp();
-      ++consumed;
-      if (lane == 0) issue(slot);
-      if (++slot == p.stages) {
-        slot = 0;
-        parity ^= 1;
-      }
-    }
-    // the warps' sums of the tile; two buffers, so that one barrier per tile is enough
-    float* mine = red + (size_t)buf * W * kOut + warp * kOut;
+      // the warp's part of this pair in this phase is complete
+      const bool has_start = begin <= pr * p.units, has_end = end >= (pr + 1) * p.units;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mine[(nt * 4 + j) * 32 + lane] = tot[nt][j];
-    __syncthreads();
-    if (p.split > 1 && joined_tile >= 0) {
-      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-      if (rank == 0) finish_join(joined_tile, buf ^ 1);
-    }
-    for (int j = tid; j < kOut; j += blockDim.x) {
-      float y = 0.f;
-      for (int w = 0; w < W; ++w) y += red[(size_t)(buf * W + w) * kOut + j];
-      const int i = j >> 5, l = j & 31;
-      const int n = (i >> 2) * 8 + (l & 3) * 2 + (i & 1), v = tile * kInt4Tile + (l >> 2) + ((i & 2) ? 8 : 0);
-      if (n < nb) y = (y * 0x1p24f) * pow2(-row_exponent(n));
-      if (p.split == 1) {
-        if (n < nb && v < p.V) int4_store(p, b0 + n, v, y);
-      } else {
-        uint32_t dst;
-        asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(dst) : "r"(smem_u32(join + (buf * p.split + rank) * kOut + j)));
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(y) : "memory");
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) tot[m][nt][j] = tot[m][nt][j] * 0x1p24f * down[nt][j & 1];
+      if (!has_start) {
+        float* mine = pieces + warp * (2 * NT * 128) + lane;
+#pragma unroll
+        for (int i = 0; i < 2 * NT * 4; ++i) {
+          const float y = tot[i / (NT * 4)][i / 4 % NT][i % 4];
+          mine[i * 32] = phase ? mine[i * 32] + y : y;
+        }
+        clear();
+        continue;
       }
+      if (p.phases > 1) {  // what the phases before left
+        float* mine = p.partial + ((size_t)blockIdx.y * (p.tiles + 1) + t_begin + pr * 2) * (NT * 128) + lane;
+#pragma unroll
+        for (int i = 0; i < 2 * NT * 4; ++i) {
+          if (t_begin + pr * 2 + i / (NT * 4) >= t_end) continue;
+          float& y = tot[i / (NT * 4)][i / 4 % NT][i % 4];
+          if (phase) y += mine[i * 32];
+          if (phase + 1 < p.phases) mine[i * 32] = y;
+        }
+      }
+      // a pair that the next warps go on with is the part's last: at the end its sums stay where they are
+      if (has_end && phase + 1 == p.phases) write_out(pr);
+      if (has_end || phase + 1 < p.phases) clear();
     }
-    if (p.split > 1) {
-      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-      joined_tile = tile;
-    }
-    buf ^= 1;
   }
-  if (p.split > 1 && joined_tile >= 0) {
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank == 0) finish_join(joined_tile, buf ^ 1);
-  }
-  if (*abort_flag && lane == 0) {
-    // a wait ran out: give copies still in flight a bounded chance to land before the CTA's memory is reused
-    for (int i = 0; i < min(issued, p.stages); ++i) {
-      const int last = ((issued - 1 - i) / p.stages) * p.stages + i;
-      mbar_wait_plain(&full[i], (uint32_t)(last / p.stages) & 1u, 100000000ull);
+  __syncthreads();
+  if (begin < end) {
+    const int pr = p_last, stop = (pr + 1) * p.units;
+    if (begin <= pr * p.units && end < stop) {
+      for (int w = warp + 1; w < W && part[w] < stop; ++w) {
+        if (part[w] == part[w + 1]) continue;
+        const float* other = pieces + w * (2 * NT * 128) + lane;
+#pragma unroll
+        for (int i = 0; i < 2 * NT * 4; ++i) tot[i / (NT * 4)][i / 4 % NT][i % 4] += other[i * 32];
+      }
+      write_out(pr);
     }
   }
 }

@@ -11,11 +11,12 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .quant import INT4_GROUPS, quantize_groups_int4
+from .quant import int4_group_ok, quantize_groups_int4
 
 __all__ = ["Int4Weight", "int4_linear"]
 
 _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
+_ws_bytes: dict[tuple, int] = {}
 
 
 class Int4Weight:
@@ -38,8 +39,8 @@ class Int4Weight:
         tiles, chunks = -(-rows // 16), -(-cols // 64)
         if qweight.dtype != torch.uint8 or qweight.shape != (tiles, chunks, 512):
             raise ValueError(f"qweight must be uint8 [{tiles}, {chunks}, 512] for a [{rows}, {cols}] weight")
-        if scales.ndim != 4 or scales.shape[1] < 1 or cols % scales.shape[1] or cols // scales.shape[1] not in INT4_GROUPS:
-            raise ValueError(f"scales must be [{tiles}, groups, 8, 2] with groups of {INT4_GROUPS} columns")
+        if scales.ndim != 4 or scales.shape[1] < 1 or cols % scales.shape[1] or not int4_group_ok(cols // scales.shape[1], cols):
+            raise ValueError(f"scales must be [{tiles}, groups, 8, 2] with groups of 32, 64 or a multiple of 128 columns")
         if scales.shape != (tiles, scales.shape[1], 8, 2):
             raise ValueError(f"scales must be [{tiles}, {scales.shape[1]}, 8, 2]")
         if scales.dtype not in (torch.bfloat16, torch.float16):
@@ -164,22 +165,27 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
             raise RuntimeError("out must not require gradients")
     if b == 0:
         return out
-    from .core import _status_word
-
     stride = x2.stride(0) if b > 1 else max(x2.stride(0), weight.cols)
     index = dev.index
     if torch._C._cuda_getDevice() == index:
-        rc = _launch(x2, stride, weight, b, out, out_stride, _status_word(dev), index)
+        rc = _launch(x2, stride, weight, b, out, out_stride, index)
     else:
         with torch.cuda.device(dev):
-            rc = _launch(x2, stride, weight, b, out, out_stride, _status_word(dev), index)
+            rc = _launch(x2, stride, weight, b, out, out_stride, index)
     if rc:
         raise _lib.FmmsError(rc, "fmms_int4_linear")
     return out
 
 
-def _launch(x, stride, weight, b, out, out_stride, status, index):
+def _launch(x, stride, weight, b, out, out_stride, index):
     qw, scales, scale_dtype, zeros, rows, cols, group = weight._args
+    key = (rows, cols, group, b)
+    nbytes = _ws_bytes.get(key)
+    if nbytes is None:
+        nbytes = _ws_bytes[key] = _lib.query_int4_workspace(*key)
+    # from torch's allocator on every call: calls on several streams, or in several captured graphs, share nothing
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     return _lib.load().fmms_int4_linear(
         x.data_ptr(), _DTYPES[x.dtype], stride, qw, scales, scale_dtype, zeros, rows, cols, group, b,
-        out.data_ptr(), _DTYPES[out.dtype], out_stride, status.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
+        out.data_ptr(), _DTYPES[out.dtype], out_stride, ws.data_ptr() if nbytes else None, nbytes,
+        torch._C._cuda_getCurrentRawStream(index))

@@ -56,7 +56,9 @@ def dequantize_rows(q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     return q.float() * scale[:, None].float()
 
 
-INT4_GROUPS = (32, 64, 128, 256)
+def int4_group_ok(group_size: int, cols: int) -> bool:
+    """Groups of 32 or 64 columns or of a multiple of 128 (up to the whole row), that divide the columns."""
+    return group_size > 0 and (group_size in (32, 64) or group_size % 128 == 0) and cols % group_size == 0
 
 
 def quantize_groups_int4(
@@ -70,8 +72,8 @@ def quantize_groups_int4(
     (default: the weight's own type if it is one of them, else bf16); codes are chosen for the rounded scale."""
     if w.ndim != 2 or not w.is_floating_point():
         raise ValueError("expected a floating-point [rows, columns] tensor")
-    if group_size not in INT4_GROUPS or w.shape[1] % group_size:
-        raise ValueError(f"group_size must be one of {INT4_GROUPS} and divide the number of columns ({w.shape[1]})")
+    if not int4_group_ok(group_size, w.shape[1]):
+        raise ValueError(f"group_size must be 32, 64 or a multiple of 128 and divide the number of columns ({w.shape[1]})")
     if scale_dtype is None:
         scale_dtype = w.dtype if w.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
     if scale_dtype not in (torch.bfloat16, torch.float16):

@@ -376,8 +376,10 @@ int fmms_static_reset(void* stream);
  *                (high nibble); rows beyond V and columns beyond D may hold anything
  *   scales       [tiles][D / group][8][2] bf16 or fp16 (rows g and 8 + g next to each other), 16-byte aligned
  *   zeros        the same shape in uint8, or NULL: 8 everywhere
- *   group        32, 64, 128 or 256, a divisor of D
+ *   group        32, 64 or a multiple of 128 (up to D: one scale per row), a divisor of D
  *   out          [B, V] bf16, fp16 or fp32, rows `out_stride` elements apart; written once, nothing else is touched
+ *   workspace    fmms_query_int4_workspace() bytes, 16-byte aligned (0 bytes, and NULL, while x fits shared memory); holds
+ *                nothing between calls, need not be zeroed, and must not be used by two calls at once
  *
  * Sums are fp32; x is brought to fp16 with an exact power of two per row (values below 2^-28 of a row's largest
  * lose bits beyond 2^-39 of it).  A row of x that is not finite gives a row that is not finite.  The order of
@@ -386,7 +388,8 @@ int fmms_static_reset(void* stream);
  */
 int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void* qweight, const void* scales,
                      int scale_dtype, const void* zeros, int V, int D, int group, int B, void* out, int out_dtype,
-                     long long out_stride, int* status_dev, void* stream);
+                     long long out_stride, void* workspace, size_t workspace_bytes, void* stream);
+int fmms_query_int4_workspace(int V, int D, int group, int B, size_t* bytes);
 
 /*
  * One step of a beam search.  For each of R requests with K beams: of all continuations (beam k, token v) the N with

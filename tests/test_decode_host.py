@@ -19,7 +19,7 @@ def _codes(rows, cols, group, zeros, seed=0):
     return q, s, z
 
 
-@pytest.mark.parametrize("rows,cols,group,zeros", [(1, 32, 32, False), (16, 64, 64, True), (17, 96, 32, True), (40, 256, 256, False), (33, 384, 128, True)])
+@pytest.mark.parametrize("rows,cols,group,zeros", [(1, 32, 32, False), (16, 64, 64, True), (17, 96, 32, True), (40, 256, 256, False), (9, 768, 768, True), (33, 384, 128, True)])
 def test_layout_follows_its_description(rows, cols, group, zeros):
     q, s, z = _codes(rows, cols, group, zeros)
     w = fs.Int4Weight.from_rows(q, s, z)
@@ -59,7 +59,7 @@ def test_quantiser_rounds_to_the_nearest_code(symmetric, dtype):
 
 def test_quantiser_refuses():
     w = torch.randn(4, 96)
-    for bad in (dict(group_size=48), dict(group_size=64), dict(group_size=512)):
+    for bad in (dict(group_size=48), dict(group_size=64), dict(group_size=512), dict(group_size=96), dict(group_size=0), dict(group_size=-32)):
         with pytest.raises(ValueError):
             quantize_groups_int4(w, **bad)
     with pytest.raises(TypeError):
@@ -85,7 +85,7 @@ def test_int4_weight_refuses_other_layouts():
     with pytest.raises(TypeError):
         fs.Int4Weight(w.qweight, w.scales.float(), w.zeros, 20, 128)
     with pytest.raises(ValueError):
-        fs.Int4Weight(w.qweight, w.scales[:, :1].expand(-1, 3, -1, -1).contiguous(), None, 20, 128)  # 3 groups of 128
+        fs.Int4Weight(w.qweight, w.scales[:, :1].expand(-1, 3, -1, -1).contiguous(), None, 20, 128)  # 128 columns in 3 groups
     with pytest.raises(ValueError):
         fs.Int4Weight(w.qweight, w.scales, w.zeros.float(), 20, 128)
     with pytest.raises(ValueError):
@@ -114,19 +114,25 @@ def test_cpu_tensors_are_refused():
 
 def test_c_entry_points_check_their_arguments(lib):
     p = 4096  # never dereferenced
-    ok = [p, 0, 64, p, p, 0, None, 100, 64, 64, 2, p, 2, 100, None, None]
+    ok = [p, 0, 64, p, p, 0, None, 100, 64, 64, 2, p, 2, 100, None, 0, None]
 
     def int4(**kw):
-        names = "x x_dtype x_stride q s s_dtype z V D group B out out_dtype out_stride status stream".split()
+        names = "x x_dtype x_stride q s s_dtype z V D group B out out_dtype out_stride ws wsb stream".split()
         return lib.fmms_int4_linear(*[kw.get(n, v) for n, v in zip(names, ok)])
 
     for kw in (dict(x=None), dict(q=None), dict(s=None), dict(out=None), dict(V=0), dict(D=0), dict(B=0), dict(B=-1),
                dict(x_dtype=2), dict(x_dtype=-1), dict(s_dtype=2), dict(out_dtype=3), dict(x_stride=63), dict(out_stride=99)):
         assert int4(**kw) == _lib.ERR_BAD_ARG, kw
-    for kw in (dict(group=48), dict(group=128), dict(group=0), dict(q=p + 8), dict(s=p + 2), dict(z=p + 4)):
+    for kw in (dict(group=48), dict(group=128), dict(group=0), dict(group=-32), dict(group=16), dict(q=p + 8), dict(s=p + 2), dict(z=p + 4)):
         assert int4(**kw) == _lib.ERR_UNSUPPORTED, kw
 
     n = ctypes.c_size_t()
+    assert lib.fmms_query_int4_workspace(151936, 4096, 128, 1, ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.fmms_query_int4_workspace(128256, 8192, 128, 16, ctypes.byref(n)) == 0 and n.value >= 128256 * 16 * 4
+    assert int4(D=8192, x_stride=8192, B=16, group=128) == _lib.ERR_WORKSPACE
+    assert int4(D=8192, x_stride=8192, B=16, group=128, ws=p, wsb=64) == _lib.ERR_WORKSPACE
+    assert lib.fmms_query_int4_workspace(100, 64, 128, 1, ctypes.byref(n)) == _lib.ERR_UNSUPPORTED
+    assert lib.fmms_query_int4_workspace(100, 64, 64, 1, None) == _lib.ERR_BAD_ARG
     assert lib.fmms_query_beam_workspace(2, 4, 1000, 8, 0, ctypes.byref(n)) == 0 and n.value >= 8 * 8 * 8
     assert lib.fmms_query_beam_workspace(2, 4, 1000, 8, 3, ctypes.byref(n)) == _lib.ERR_BAD_ARG
     assert lib.fmms_query_beam_workspace(2, 4, 1000, 65, 0, ctypes.byref(n)) == _lib.ERR_UNSUPPORTED

@@ -265,7 +265,7 @@ def test_reorder(fs, R, K, rest, dtype):
     for dim, shape in ((0, (R * K, *rest)), (1, (6, R * K, *rest)), (2, (2, 3, R * K, *rest))):
         state = _fill(shape, dtype, seed=K)
         want = _reordered(state, parents, dim)
-        assert fs.reorder_beams(state, parents, dim=dim) is None
+        assert fs.reorder_beams(state, parents, dim=dim, length_dim=dim + 1) is None  # no lengths: whole beams
         assert _same(state, want)
 
 
@@ -352,7 +352,7 @@ def test_reorder_refusals(fs):
         (dict(parents=parents.float()), ValueError), (dict(parents=parents[0]), ValueError), (dict(states=s[:5]), ValueError),
         (dict(states=s[:1].expand(6, 4, 5)), ValueError), (dict(states=[s, s]), ValueError), (dict(states=s.cpu()), RuntimeError),
         (dict(parents=parents.cpu()), RuntimeError), (dict(dim=3), ValueError), (dict(dim=1), ValueError), (dict(lengths=lengths), ValueError),
-        (dict(length_dim=1), ValueError), (dict(lengths=lengths, length_dim=0), ValueError), (dict(lengths=lengths[:1], length_dim=1), ValueError),
+        (dict(lengths=lengths, length_dim=0), ValueError), (dict(lengths=lengths[:1], length_dim=1), ValueError),
         (dict(lengths=lengths.float(), length_dim=1), ValueError), (dict(lengths=lengths, length_dim=1, states=s.transpose(1, 2)), ValueError),
         (dict(states=torch.zeros(6, 4, device=_dev(), requires_grad=True)), RuntimeError),
         (dict(states=torch.zeros(65, 4, device=_dev()), parents=torch.zeros(1, 65, dtype=torch.int64, device=_dev())), ValueError),
@@ -380,14 +380,15 @@ def _plain_search(step_logits, R, K, steps, eos, pad):
     return beams
 
 
+@pytest.mark.parametrize("eos", [7, 38, 191])  # on the CPU: no beam, one beam, three beams finish
 @pytest.mark.parametrize("kind", ["bf16", "int4", "fp8"])
-def test_search_on_every_head(fs, kind):
+def test_search_on_every_head(fs, kind, eos):
     """Heads, selection, history, finished beams and states together: a toy language model whose hidden state is an
     embedding of the last two tokens, kept as a per-beam state that the search reorders."""
     from flashsampling_b200.quant import dequantize_rows, quantize_rows_e4m3
     from oracle import fmms_oracle as O
 
-    R, K, V, D, steps, eos, pad = 3, 4, 200, 64, 6, 7, 1
+    R, K, V, D, steps, pad = 3, 4, 200, 64, 6, 1
     g = torch.Generator().manual_seed(11)
     w = (torch.randn(V, D, generator=g) * 0.35).bfloat16()
     w[eos] += 0.05
@@ -422,15 +423,15 @@ def test_search_on_every_head(fs, kind):
         state.copy_(h)
     fs.check_status()
     got_t, got_s = search.tokens.view(R, K, steps).cpu(), search.scores.cpu()
-    any_finished = False
+    ended = 0
     for r in range(R):
         for k in range(K):
             toks, sc, fin = want[r][k]
             assert got_t[r, k].tolist() == list(toks)
             assert abs(float(got_s[r, k]) - sc) < 1e-3 * steps  # logits within 1e-4 of their scale on every head
             assert bool(search.finished[r, k]) == fin
-            any_finished |= fin
-    assert any_finished
+            ended += fin
+    assert ended == {7: 0, 38: 1, 191: 3}[eos]
     tokens, score = search.best(length_penalty=1.0)
     for r in range(R):
         ranked = [s / (toks.index(eos) + 1 if eos in toks else steps) for toks, s, _ in want[r]]

@@ -73,6 +73,22 @@ def test_against_the_dequantised_weight(fs, rows, cols, batch, group, zeros):
     fs.check_status()
 
 
+@pytest.mark.parametrize("cols,group", [(640, 640), (2688, 384), (5376, 2688), (9216, 512)])
+def test_groups_of_many_columns(fs, cols, group):
+    w = _weight(fs, 170, cols, group, True, seed=cols)
+    x = _x(9, cols, torch.bfloat16)
+    want, bound = _reference(w, x)
+    _check(fs.int4_linear(x, w, out_dtype=torch.float32), want, bound)
+
+
+@pytest.mark.parametrize("cols", [64, 192, 320])
+def test_half_filled_last_fetch(fs, cols):
+    w = _weight(fs, 70, cols, 64, True, seed=cols)
+    x = _x(3, cols, torch.bfloat16)
+    want, bound = _reference(w, x)
+    _check(fs.int4_linear(x, w, out_dtype=torch.float32), want, bound)
+
+
 @pytest.mark.parametrize("cols", [32, 96, 160, 4128])
 def test_half_filled_last_chunk(fs, cols):
     w = _weight(fs, 130, cols, 32, True, seed=cols)
@@ -93,14 +109,15 @@ def test_types(fs, xt, st, ot):
 
 
 @pytest.mark.parametrize("rows,cols,batch,group", [
-    (40, 16384, 1, 128),  # few tiles, long rows: a cluster per tile
+    (40, 16384, 1, 128),  # few tiles, long rows
     (40, 16384, 16, 128),
     (9000, 8192, 16, 128),  # x of 16 rows does not fit one CTA
     (3000, 16384, 30, 64),
     (500, 28672, 8, 256),
-    (48, 65536, 9, 256),  # falls back to fewer rows per pass
+    (48, 65536, 9, 256),
+    (16, 256 * 1024, 1, 256),
 ])
-def test_columns_split_over_a_cluster(fs, rows, cols, batch, group):
+def test_columns_in_phases(fs, rows, cols, batch, group):
     w = _weight(fs, rows, cols, group, True, seed=rows)
     x = _x(batch, cols, torch.bfloat16)
     want, bound = _reference(w, x)
@@ -242,6 +259,3 @@ def test_refusals(fs):
         fs.int4_linear(x.clone().requires_grad_(), w)
     with torch.no_grad():
         fs.int4_linear(x.clone().requires_grad_(), w)
-    big = _weight(fs, 16, 256 * 1024, 256, False)
-    with pytest.raises(fs._lib.FmmsError, match="unsupported"):
-        fs.int4_linear(_x(1, 256 * 1024, torch.bfloat16), big)  # a row of x does not fit eight CTAs

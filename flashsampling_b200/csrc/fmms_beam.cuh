@@ -2,14 +2,17 @@
 //   total[k, v] = score[k] + x[k, v] - ln sum_v exp x[k, v],
 // equal totals in the order of (k, v).
 //
-// Two kernels.  beam_part_kernel reads the logits once: a CTA holds a slice of one row in registers, takes its maximum,
-// its sum of exponentials and its N largest logits (within a row the order of the totals is the order of the logits).
+// Two kernels.  beam_part_kernel reads the logits once: a CTA streams a slice of one row through a ring of asynchronous
+// copies (each thread reads back only what it copied itself, so the loop has no barrier) and keeps the slice's maximum, its
+// sum of exponentials and its N largest logits - within a row the order of the totals is the order of the logits.
 // beam_merge_kernel, one CTA per request, joins the slices' sums and picks the N best of what they kept.
 //
 // The N largest of a set are found through a bound: split the set into G >= N groups; the N-th largest of the groups'
 // maxima cannot exceed the N-th largest element.  What reaches the bound is N elements and, with random order, few more
-// (G = 32: 9.2 of 8, 22 of 16); they are counted against each other for their ranks.  Where more reach it than the
-// list holds (many equal logits), the N largest are taken one after the other.
+// (G = 32: 9.2 of 8, 22 of 16).  A slice takes a first bound from its first quarter and notes the vectors with an element
+// that reaches it; the final bound, from the whole slice, picks the elements, which are counted against each other for
+// their ranks.  Where the first bound leaves too many vectors (tokens masked there, logits that rise), all are looked at
+// again; where the final one leaves too many elements (many equal logits), the N largest are taken one after the other.
 //
 // Two beams' candidates may lie arbitrarily close, and their order is an integer output, so sums and totals are formed
 // to more than 32 bits: exponentials carry the rounding of their argument along, slices join in fp64, and totals are
@@ -18,23 +21,29 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "fmms_common.cuh"
 
 namespace fmms {
 
 constexpr int kBeamThreads = 256;
-constexpr int kBeamVecs = 4;         // 16-byte loads of a thread: the slice of a CTA is 16 KiB
-constexpr int kBeamMaxN = 64;        // candidates
-constexpr int kBeamMaxK = 64;        // beams
-constexpr int kBeamListCap = 512;    // elements of a slice that reach the bound
-constexpr int kBeamMergeCap = 1024;  // the same over a request
+constexpr int kBeamMaxN = 64;       // candidates
+constexpr int kBeamMaxK = 64;       // beams
+constexpr int kBeamRing = 6;        // 16-byte vectors a thread has in flight or in hand
+constexpr int kBeamFirst = 4;       // vectors of a thread that the bound is taken from
+constexpr int kBeamMaxIters = 16;   // vectors of a thread in a slice
+constexpr int kBeamVecCap = 768;    // vectors of a slice with an element that reaches the first bound
+constexpr int kBeamListCap = 512;   // elements of a slice that reach the final bound
+constexpr int kBeamItems = 1024;    // entries that the merge holds at a time
+constexpr int kBeamMergeCap = kBeamItems + kBeamMaxN;
 
 struct BeamParams {
   const void* logits;          // row (r, k) at r * stride_r + k * stride_k elements
   long long stride_r, stride_k;
   const float* scores;         // [R, K]
   const uint8_t* finished;     // [R, K] or null
-  int R, K, V, N, splits;
+  int R, K, V, N, splits, iters;  // iters: vectors of a thread in a slice
   long long pad_token;
   unsigned long long* keys;    // [R * K][splits][N] (value, index), descending; 0: none
   double* sums;                // [R * K][splits] sum of exp(x - max)
@@ -55,25 +64,27 @@ __device__ __forceinline__ float2 beam_pair<__half>(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-// the elements of a 16-byte vector as fp32
+// pair i of the elements of a 16-byte vector, as fp32
 template <typename T>
-__device__ __forceinline__ void beam_unpack(const uint4& u, float (&v)[16 / sizeof(T)]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 4) {
-      v[i] = __uint_as_float(w[i]);
-    } else {
-      const float2 f = beam_pair<T>(w[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
-  }
+__device__ __forceinline__ float2 beam_get(const uint4& u, int i) {
+  if constexpr (sizeof(T) == 4)
+    return i == 0 ? make_float2(__uint_as_float(u.x), __uint_as_float(u.y)) : make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+  else
+    return beam_pair<T>(i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w);
 }
 
+// the largest element of a vector; NaN never is (nor does it turn up when all are NaN: the result is then -inf)
 template <typename T>
-__host__ __device__ constexpr int beam_tile() {
-  return kBeamThreads * kBeamVecs * (int)(16 / sizeof(T));
+__device__ __forceinline__ float beam_vec_max(const uint4& u) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w))), -INFINITY);
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* h = reinterpret_cast<const T2*>(&u);
+    const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    const float2 f = beam_pair<T>(*reinterpret_cast<const uint32_t*>(&m));
+    return fmaxf(fmaxf(f.x, f.y), -INFINITY);
+  }
 }
 
 __device__ __forceinline__ bool beam_live(const BeamParams& p, int row) {
@@ -81,140 +92,266 @@ __device__ __forceinline__ bool beam_live(const BeamParams& p, int row) {
   return s - s == 0.f;  // neither infinite nor NaN
 }
 
+// e^x for x <= 0 to some 1e-12 relative: 2^k times the Taylor polynomial of the rest (|rest| <= ln 2 / 2, rest^11 / 11! <
+// 3e-13).  Small where a library call is some hundred instructions, which a kernel of a few microseconds first has to fetch.
+__device__ __forceinline__ double beam_exp(double x) {
+  if (!(x > -700.)) return 0.;
+  const double k = rint(x * 1.4426950408889634), r = fma(k, -0.6931471805599453, x);
+  double y = 1. / 3628800.;
+  y = fma(y, r, 1. / 362880.);
+  y = fma(y, r, 1. / 40320.);
+  y = fma(y, r, 1. / 5040.);
+  y = fma(y, r, 1. / 720.);
+  y = fma(y, r, 1. / 120.);
+  y = fma(y, r, 1. / 24.);
+  y = fma(y, r, 1. / 6.);
+  y = fma(y, r, 0.5);
+  y = fma(y, r, 1.);
+  y = fma(y, r, 1.);
+  return y * __hiloint2double(((int)k + 1023) << 20, 0);
+}
+
+// ln x for x >= 1: the fp32 logarithm and one Newton step, y + (x e^-y - 1), whose error is the square of fp32's
+__device__ __forceinline__ double beam_log(double x) {
+  const double y = (double)logf((float)x);
+  return y + fma(x, beam_exp(-y), -1.);
+}
+
+// The n-th largest of 32 values, one per lane (equal ones in the order of the lanes).
+__device__ __forceinline__ float warp_nth(float v, int n) {
+  const int lane = threadIdx.x & 31;
+  int rank = 0;
+#pragma unroll 8
+  for (int i = 0; i < 32; ++i) {
+    const float o = __shfl_sync(0xffffffffu, v, i);
+    rank += o > v || (o == v && i < lane);
+  }
+  return __shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, rank == n - 1)) - 1);
+}
+
+// The same of 128 values, four per lane.
+__device__ __noinline__ float warp_nth4(float4 v4, int n) {
+  const int lane = threadIdx.x & 31;
+  const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+  int rank[4] = {0, 0, 0, 0};
+#pragma unroll 1
+  for (int i = 0; i < 32; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float o = __shfl_sync(0xffffffffu, v[q], i);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) rank[r] += o > v[r] || (o == v[r] && q * 32 + i < r * 32 + lane);
+    }
+  float found = -INFINITY;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const unsigned b = __ballot_sync(0xffffffffu, rank[r] == n - 1);
+    if (b) found = __shfl_sync(0xffffffffu, v[r], __ffs(b) - 1);
+  }
+  return found;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kBeamThreads) beam_part_kernel(const BeamParams p) {
+__global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamParams p) {
   constexpr int VE = 16 / sizeof(T);
+  __shared__ __align__(16) uint4 ring[kBeamRing][kBeamThreads];
   __shared__ __align__(16) float gmax[128];
   __shared__ float sh_pivot;
-  __shared__ int sh_count;
+  __shared__ int sh_vecs, sh_count;
+  __shared__ int vec_list[kBeamVecCap];
   __shared__ unsigned long long list[kBeamListCap];
-  __shared__ double wsum[kBeamThreads / 32];
+  __shared__ double wsum[kBeamThreads / 32], wsum_up[kBeamThreads / 32];
   __shared__ unsigned long long wbest[kBeamThreads / 32];
   griddep_launch_dependents();
   const int row = blockIdx.y, split = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if ((p.finished && p.finished[row]) || !beam_live(p, row)) return;  // the merge does not look at such rows either
   const T* x = reinterpret_cast<const T*>(p.logits) + (row / p.K) * p.stride_r + (row % p.K) * p.stride_k;
-  const int lead = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));  // elements back to a 16-byte boundary
-  const int first = split * beam_tile<T>() + tid * VE - lead;  // index of the thread's first element (may be < 0)
+  // whole vectors on 16-byte boundaries, behind up to VE - 1 elements before the first boundary and before as many at the
+  // end: the first and the last slice's single elements
+  const int lead = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T), p.V);
+  const int vecs = (p.V - lead) / VE, tail = lead + vecs * VE;
+  const int v_begin = min(split * p.iters * kBeamThreads, vecs), v_end = min(v_begin + p.iters * kBeamThreads, vecs);
+  const int singles = (split == 0 ? lead : 0) + (split == p.splits - 1 ? p.V - tail : 0);
+  const T* xv = x + lead;
 
-  uint4 u[kBeamVecs];
+  auto fetch = [&](int v, int slot) {  // vector v of the row, for this thread
+    if (v < v_end)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&ring[slot][tid])), "l"(xv + (size_t)v * VE) : "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
 #pragma unroll
-  for (int j = 0; j < kBeamVecs; ++j) {
-    const int i = first + j * kBeamThreads * VE;
-    if (i >= 0 && i + VE <= p.V) {
-      u[j] = __ldg(reinterpret_cast<const uint4*>(x + i));
+  for (int i = 0; i < kBeamRing - 1; ++i) fetch(v_begin + i * kBeamThreads + tid, i);
+  float single = -INFINITY;
+  int single_at = 0;
+  if (tid < singles) {  // at most 2 (VE - 1) threads
+    const int head = split == 0 ? lead : 0;
+    single_at = tid < head ? tid : tail + tid - head;
+    single = fmaxf((float)x[single_at], -INFINITY);
+  }
+  if (tid == 0) sh_vecs = sh_count = 0;
+
+  // bound and first reference of the exponentials from the first vectors (fmaxf drops NaN)
+  asm volatile("cp.async.wait_group %0;" ::"n"(kBeamRing - 1 - kBeamFirst) : "memory");
+  float m = single;
+#pragma unroll 1
+  for (int i = 0; i < kBeamFirst; ++i)
+    if (v_begin + i * kBeamThreads + tid < v_end) m = fmaxf(m, beam_vec_max<T>(ring[i][tid]));
+  // The N-th largest of 32 groups' maxima (8 lanes each; up to 32 candidates), or of 128 (2 lanes): into sh_pivot; the
+  // largest: returned.
+  const bool wide = p.N <= 32;
+  auto bound = [&](float m) {
+    float gm = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    if (wide) {
+      gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 2));
+      gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 4));
+    }
+    const int shift = wide ? 3 : 1;
+    if ((tid & ((1 << shift) - 1)) == 0) gmax[tid >> shift] = gm;
+    __syncthreads();
+    float top = gmax[lane];
+    if (wide) {
+      if (warp == 0) {
+        const float v = warp_nth(top, p.N);
+        if (lane == 0) sh_pivot = v;
+      }
     } else {
-      alignas(16) T e[VE];
-#pragma unroll
-      for (int q = 0; q < VE; ++q) e[q] = (i + q >= 0 && i + q < p.V) ? x[i + q] : (T)(-INFINITY);
-      u[j] = *reinterpret_cast<const uint4*>(e);
+      const float4 v4 = make_float4(top, gmax[lane + 32], gmax[lane + 64], gmax[lane + 96]);
+      top = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
+      if (warp == 0) {
+        const float v = warp_nth4(v4, p.N);
+        if (lane == 0) sh_pivot = v;
+      }
     }
-  }
-  float m = -INFINITY;  // fmaxf drops NaN
 #pragma unroll
-  for (int j = 0; j < kBeamVecs; ++j) {
-    float v[VE];
-    beam_unpack<T>(u[j], v);
-#pragma unroll
-    for (int q = 0; q < VE; ++q) m = fmaxf(m, v[q]);
-  }
-  // groups of 8 lanes (32 groups) or of 2 lanes (128 groups)
-  const int wide = p.N <= 16;
-  float gm = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  if (wide) {
-    gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 2));
-    gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 4));
-  }
-  const int G = wide ? 32 : 128, per = kBeamThreads / G;
-  if (tid % per == 0) gmax[tid / per] = gm;
-  if (tid == 0) sh_count = 0;
-  __syncthreads();
-  float top = -INFINITY;
-  for (int i = lane; i < G; i += 32) top = fmaxf(top, gmax[i]);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  if (tid < G) {
-    const float v = gmax[tid];
-    int rank = 0;
-    for (int i = 0; i < G; i += 4) {
-      const float4 o = *reinterpret_cast<const float4*>(&gmax[i]);
-      rank += (o.x > v || (o.x == v && i < tid)) + (o.y > v || (o.y == v && i + 1 < tid)) +
-              (o.z > v || (o.z == v && i + 2 < tid)) + (o.w > v || (o.w == v && i + 3 < tid));
-    }
-    if (rank == p.N - 1) sh_pivot = v;
-  }
-  // sum of exp(x - top): 2^(hi + lo) with hi + lo = (x - top) log2(e) to twice the precision, 2^lo = 1 + lo ln 2.
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    __syncthreads();
+    return top;
+  };
+  const float ref0 = bound(m);
+  float pivot = sh_pivot;
+
+  // sum of exp(x - ref): 2^(hi + lo) with hi + lo = (x - ref) log2(e) to twice the precision, 2^lo = 1 + lo ln 2.
   // The bound of -200 gives 0 and also stands in for -inf, and for NaN, which fmaxf drops.
-  constexpr float kL = kLog2e, kL2 = 1.9259629911266175e-8f;  // log2(e) = kL + kL2
-  float s = 0.f, c = 0.f;
-#pragma unroll
-  for (int j = 0; j < kBeamVecs; ++j) {
-    float v[VE];
-    beam_unpack<T>(u[j], v);
-#pragma unroll
-    for (int q = 0; q < VE; ++q) {
-      const float d = fmaxf(v[q] - top, -200.f);
-      const float hi = d * kL;
-      const float lo = fmaf(d, kL2, fmaf(d, kL, -hi));
-      const float e = ex2_approx(hi);
-      s += e;
-      c = fmaf(e, lo, c);
-    }
+  constexpr float kRest = 1.92596299e-8f;  // log2(e) = kLog2e + kRest
+  const float2 kL = make_float2(kLog2e, kLog2e), kNegL = make_float2(-kLog2e, -kLog2e), kNegRest = make_float2(-kRest, -kRest);
+  float ref = ref0;
+  float2 s = make_float2(0.f, 0.f), c = make_float2(0.f, 0.f);  // sums of e, and of e times minus lo
+  auto add = [&](float2 v) {
+    float2 d = __fadd2_rn(v, make_float2(-ref, -ref));
+    d.x = fmaxf(d.x, -200.f);
+    d.y = fmaxf(d.y, -200.f);
+    const float2 hi = __fmul2_rn(d, kL);
+    const float2 lo = __ffma2_rn(d, kNegRest, __ffma2_rn(d, kNegL, hi));
+    const float2 e = make_float2(ex2_approx(hi.x), ex2_approx(hi.y));
+    s = __fadd2_rn(s, e);
+    c = __ffma2_rn(e, lo, c);
+  };
+  double before = 0.;  // the sum from before the last rise of the reference, in its units
+  auto sum_now = [&] { return before + ((double)s.x + (double)s.y) - ((double)c.x + (double)c.y) * 0.6931471805599453; };
+  auto raise = [&](float to) {
+    const double sum = sum_now();
+    before = sum == 0. ? 0. : sum * beam_exp((double)ref - (double)to);
+    s = make_float2(0.f, 0.f);
+    c = make_float2(0.f, 0.f);
+    ref = to;
+  };
+  if (tid < singles) {
+    add(make_float2(single, -INFINITY));  // not above ref
   }
-  double sum = (double)s + (double)c * 0.6931471805599453;
+  const uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -inf
+  int slot = 0, next = kBeamRing - 1;
+#pragma unroll 1
+  for (int i = 0, v = v_begin + tid; i < p.iters; ++i, v += kBeamThreads) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kBeamRing - 2) : "memory");
+    uint4 u = make_uint4(kNone, kNone, kNone, kNone);
+    if (v < v_end) u = ring[slot][tid];
+    fetch(v + (kBeamRing - 1) * kBeamThreads, next);
+    const float vm = beam_vec_max<T>(u);
+    m = fmaxf(m, vm);
+    // rare, and left together: the exponentials below are the warp's again
+    if (vm > ref) raise(vm);
+    if (vm >= pivot && vm > -INFINITY) {
+      const int pos = atomicAdd(&sh_vecs, 1);
+      if (pos < kBeamVecCap) vec_list[pos] = v;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < VE / 2; ++q) add(beam_get<T>(u, q));
+    if (++slot == kBeamRing) slot = 0;
+    if (++next == kBeamRing) next = 0;
+  }
+  const double mine = sum_now();
+  float top = ref0;
+  if (p.iters > kBeamFirst) {  // else the first bound is that of the whole slice
+    top = bound(m);
+    pivot = sh_pivot;
+  } else {
+    __syncthreads();  // the noted vectors are complete
+  }
+  // threads whose reference is still the first one add up in its units, the others in those of the slice's maximum
+  double sum = ref == ref0 ? mine : 0., sum_up = 0.;
+  if (ref != ref0 && mine > 0.) sum_up = mine * beam_exp((double)ref - (double)top);
+  const bool any_up = __any_sync(0xffffffffu, sum_up > 0.);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-  if (lane == 0) wsum[warp] = sum;
-  __syncthreads();
-  const float pivot = sh_pivot;
-  if (m >= pivot && m > -INFINITY) {
+  if (any_up)
 #pragma unroll
-    for (int j = 0; j < kBeamVecs; ++j) {
-      float v[VE];
-      beam_unpack<T>(u[j], v);
-#pragma unroll
-      for (int q = 0; q < VE; ++q)
-        if (v[q] >= pivot && v[q] > -INFINITY) {
-          const int pos = atomicAdd(&sh_count, 1);
-          // + 0.f: -0 counts as 0
-          if (pos < kBeamListCap) list[pos] = cand_key(v[q] + 0.f, first + j * kBeamThreads * VE + q);
-        }
-    }
+    for (int off = 16; off > 0; off >>= 1) sum_up += __shfl_xor_sync(0xffffffffu, sum_up, off);
+  if (lane == 0) {
+    wsum[warp] = sum;
+    wsum_up[warp] = sum_up;
   }
+  // the elements that reach the bound: of the noted vectors, or of all where too many were noted
+  auto offer = [&](float v, int at) {
+    if (v >= pivot && v > -INFINITY) {
+      const int pos = atomicAdd(&sh_count, 1);
+      if (pos < kBeamListCap) list[pos] = cand_key(v + 0.f, at);  // + 0.f: -0 counts as 0
+    }
+  };
+  const bool noted = sh_vecs <= kBeamVecCap;
+  const int look = (noted ? sh_vecs : v_end - v_begin) * VE;
+#pragma unroll 1
+  for (int i = tid; i < look; i += kBeamThreads) {
+    const int at = lead + (noted ? vec_list[i / VE] : v_begin + i / VE) * VE + i % VE;
+    offer((float)x[at], at);
+  }
+  if (tid < singles) offer(single, single_at);
   __syncthreads();
   const int n = sh_count;
   const size_t part = (size_t)row * p.splits + split;
   unsigned long long* out = p.keys + part * p.N;
-  if (tid == 0) {
-    double total = 0.;
-    for (int w = 0; w < kBeamThreads / 32; ++w) total += wsum[w];
-    p.sums[part] = total;
+  if (tid == kBeamThreads - 1) {  // the last warp: the first ones rank the list
+    double all = 0., up = 0.;
+    for (int w = 0; w < kBeamThreads / 32; ++w) {
+      all += wsum[w];
+      up += wsum_up[w];
+    }
+    p.sums[part] = (ref0 == top || all == 0. ? all : all * beam_exp((double)ref0 - (double)top)) + up;
     p.maxima[part] = top;
   }
   if (n <= kBeamListCap) {
     for (int i = tid; i < n; i += kBeamThreads) {
       const unsigned long long key = list[i];
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < n; ++j) rank += list[j] > key;
       if (rank < p.N) out[rank] = key;
     }
     for (int i = n + tid; i < p.N; i += kBeamThreads) out[i] = 0ull;
     return;
   }
-  // many elements at the bound: one maximum after the other (keys differ, each is below the last)
+  // many elements at the bound: one maximum after the other (keys differ, each is below the last), read again
+  const int from = split == 0 ? 0 : lead + v_begin * VE, to = split == p.splits - 1 ? p.V : lead + v_end * VE;
   unsigned long long last = ~0ull;
   for (int r = 0; r < p.N; ++r) {
     unsigned long long best = 0ull;
-#pragma unroll
-    for (int j = 0; j < kBeamVecs; ++j) {
-      float v[VE];
-      beam_unpack<T>(u[j], v);
-#pragma unroll
-      for (int q = 0; q < VE; ++q)
-        if (v[q] > -INFINITY) {
-          const unsigned long long key = cand_key(v[q] + 0.f, first + j * kBeamThreads * VE + q);
-          if (key < last && key > best) best = key;
-        }
+#pragma unroll 1
+    for (int i = from + tid; i < to; i += kBeamThreads) {
+      const float v = (float)x[i];
+      if (v > -INFINITY) {
+        const unsigned long long key = cand_key(v + 0.f, i);
+        if (key < last && key > best) best = key;
+      }
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, off));
@@ -227,165 +364,159 @@ __global__ void __launch_bounds__(kBeamThreads) beam_part_kernel(const BeamParam
   }
 }
 
-struct BeamCand {
-  double total;
-  unsigned int at;  // k * V + v
-};
 __device__ __forceinline__ bool beam_before(double t1, unsigned int a1, double t2, unsigned int a2) {
   return t1 > t2 || (t1 == t2 && a1 < a2);
 }
 
+// One CTA per request.  What the slices kept is a set of lists, K * splits of them with N entries each.  Up to 1024
+// entries at a time, joined with the best N of the ones before, shrink to what reaches their bound (again and again
+// while they are many) and are counted against each other.
 __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamParams p) {
   __shared__ double lse[kBeamMaxK], base[kBeamMaxK];
-  __shared__ int kind[kBeamMaxK];  // 0: no candidates, 1: its list, 2: finished (one candidate)
-  __shared__ double tmax[kBeamThreads];
-  __shared__ double sh_pivot;
-  __shared__ int sh_count;
-  __shared__ double list_t[kBeamMergeCap];
-  __shared__ unsigned int list_a[kBeamMergeCap];
+  __shared__ int kind[kBeamMaxK];  // 0: no candidates, 1: its lists, 2: finished (one candidate)
+  __shared__ double list_t[2][kBeamMergeCap];
+  __shared__ unsigned int list_a[2][kBeamMergeCap];
+  __shared__ float gmax[kBeamThreads];
+  __shared__ int sh_count[2];
   griddep_wait();  // launched behind beam_part_kernel with programmatic stream serialisation
   const int r = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) {
-    sh_count = 0;
-    sh_pivot = -INFINITY;
-  }
+  const int per_row = p.splits * p.N, items = p.K * per_row;
+  const unsigned long long* keys = p.keys + (size_t)r * items;
+  const size_t o = (size_t)r * p.N;
+
+  // the first entries (of rows without lists: whatever is there, not looked at) come while the sums do
+  const unsigned long long early0 = tid < items ? __ldcg(keys + tid) : 0ull;
+  const unsigned long long early1 = tid + kBeamThreads < items ? __ldcg(keys + tid + kBeamThreads) : 0ull;
+
+  // the beams' log-sum-exps: a warp per beam
+#pragma unroll 1
   for (int k = warp; k < p.K; k += kBeamThreads / 32) {
-    const int row = r * p.K + k;
-    const bool live = beam_live(p, row), done = p.finished && p.finished[row];
+    const int at = r * p.K + k;
+    const float score = p.scores[at];
+    const bool live = score - score == 0.f, done = p.finished && p.finished[at];
     double S = 0.;
     float mx = -INFINITY;
     if (live && !done) {
-      for (int i = lane; i < p.splits; i += 32) mx = fmaxf(mx, p.maxima[(size_t)row * p.splits + i]);
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-      if (mx - mx == 0.f) {
-        for (int i = lane; i < p.splits; i += 32) {
-          const float mi = p.maxima[(size_t)row * p.splits + i];
-          if (mi > -INFINITY) S += p.sums[(size_t)row * p.splits + i] * exp((double)mi - (double)mx);
+#pragma unroll 1
+      for (int i0 = 0; i0 < p.splits; i0 += 32) {
+        const int i = i0 + lane;
+        float mi = -INFINITY;
+        double si = 0.;
+        if (i < p.splits) {
+          mi = p.maxima[(size_t)at * p.splits + i];
+          si = p.sums[(size_t)at * p.splits + i];
         }
+        float all = fmaxf(mi, mx);
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) S += __shfl_xor_sync(0xffffffffu, S, off);
+        for (int off = 16; off > 0; off >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, off));
+        double term = mi > -INFINITY ? si * beam_exp((double)mi - (double)all) : 0.;
+        if (i0 > 0 && lane == 0 && mx > -INFINITY) term += S * beam_exp((double)mx - (double)all);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) term += __shfl_xor_sync(0xffffffffu, term, off);
+        S = term;
+        mx = all;
       }
     }
     if (lane == 0) {
-      base[k] = (double)p.scores[row];
+      base[k] = (double)score;
       kind[k] = !live ? 0 : done ? 2 : (mx - mx == 0.f) ? 1 : 0;
-      lse[k] = kind[k] == 1 ? (double)mx + log(S) : 0.;
+      lse[k] = kind[k] == 1 ? (double)mx + beam_log(S) : 0.;
     }
   }
-  __syncthreads();
-  const int per_row = p.splits * p.N, E = p.K * per_row;
-  // entry e of the request; false: none
-  auto entry = [&](int e, double& t, unsigned int& a) {
-    const int k = e / per_row;
-    if (kind[k] == 1) {
-      const unsigned long long key = p.keys[((size_t)r * p.K) * per_row + e];
-      if (key == 0ull) return false;
-      float v;
-      int idx;
-      cand_key_decode(key, v, idx);
-      t = base[k] + ((double)v - lse[k]);
-      a = (unsigned int)k * (unsigned int)p.V + (unsigned int)idx;
-      return true;
-    }
-    if (kind[k] == 2 && e == k * per_row) {
-      t = base[k];
-      a = (unsigned int)k * (unsigned int)p.V + (unsigned int)p.pad_token;
-      return true;
-    }
-    return false;
-  };
-  double m = -INFINITY;
-  for (int e = tid; e < E; e += kBeamThreads) {
-    double t;
-    unsigned int a;
-    if (entry(e, t, a)) m = fmax(m, t);
-  }
-  tmax[tid] = m;
-  __syncthreads();
-  const int G = p.N <= 16 ? 32 : kBeamThreads;  // groups: equal lanes of the warps, or single threads
-  if (G == 32 && tid < 32) {
-    for (int w = 1; w < kBeamThreads / 32; ++w) m = fmax(m, tmax[w * 32 + tid]);
-    __syncwarp();
-    tmax[tid] = m;
-    __syncwarp();
-  }
-  if (tid < G) {
-    int rank = 0;
-    for (int i = 0; i < G; ++i) rank += tmax[i] > m || (tmax[i] == m && i < tid);
-    if (rank == p.N - 1) sh_pivot = m;
-  }
-  __syncthreads();
-  const double pivot = sh_pivot;
-  for (int e = tid; e < E; e += kBeamThreads) {
-    double t;
-    unsigned int a;
-    if (entry(e, t, a) && t >= pivot) {
-      const int pos = atomicAdd(&sh_count, 1);
-      if (pos < kBeamMergeCap) {
-        list_t[pos] = t;
-        list_a[pos] = a;
+  int cur = 0, have = 0;  // the list in use; the best candidates so far, at its front
+#pragma unroll 1
+  for (int first = 0; first < items; first += kBeamItems) {
+    if (tid == 0) sh_count[cur] = have;
+    __syncthreads();
+    const int last = min(items, first + kBeamItems);
+#pragma unroll 1
+    for (int j = 0, i = first + tid; i < last; ++j, i += kBeamThreads) {
+      const int k = i / per_row;
+      const unsigned long long key = first == 0 && j < 2 ? (j == 0 ? early0 : early1) : __ldcg(keys + i);
+      double t;
+      unsigned int a;
+      if (kind[k] == 1) {
+        if (key == 0ull) continue;
+        float v;
+        int idx;
+        cand_key_decode(key, v, idx);
+        t = base[k] + ((double)v - lse[k]);
+        a = (unsigned int)k * (unsigned int)p.V + (unsigned int)idx;
+      } else if (kind[k] == 2 && i == k * per_row) {
+        t = base[k];
+        a = (unsigned int)k * (unsigned int)p.V + (unsigned int)p.pad_token;
+      } else {
+        continue;
       }
+      const int pos = atomicAdd(&sh_count[cur], 1);
+      list_t[cur][pos] = t;
+      list_a[cur][pos] = a;
     }
-  }
-  __syncthreads();
-  const int n = sh_count;
-  const size_t o = (size_t)r * p.N;
-  auto put = [&](int rank, double t, unsigned int a) {
-    p.out_scores[o + rank] = (float)t;
-    p.out_tokens[o + rank] = (long long)(a % (unsigned int)p.V);
-    p.out_parents[o + rank] = (long long)(a / (unsigned int)p.V);
-  };
-  int found = min(n, p.N);
-  if (n <= kBeamMergeCap) {
-    for (int i = tid; i < n; i += kBeamThreads) {
-      const double t = list_t[i];
-      const unsigned int a = list_a[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += beam_before(list_t[j], list_a[j], t, a);
-      if (rank < p.N) put(rank, t, a);
-    }
-  } else {
-    // one after the other: the best entry behind the last one taken
-    double lt = INFINITY;
-    unsigned int la = 0u;
-    for (int i = 0; i < p.N; ++i) {
-      double bt = -INFINITY;
-      unsigned int ba = 0xffffffffu;
-      for (int e = tid; e < E; e += kBeamThreads) {
-        double t;
-        unsigned int a;
-        if (entry(e, t, a) && (i == 0 || beam_before(lt, la, t, a)) && beam_before(t, a, bt, ba)) {
-          bt = t;
-          ba = a;
-        }
-      }
+    __syncthreads();
+    int n = sh_count[cur];
+    // Keep what reaches the N-th largest of the maxima of 32 (or 128) groups, item i in group i mod 32 (128).  Rounded
+    // down to fp32 the totals keep their order, and a bound need not tell apart what rounding makes equal.
+#pragma unroll 1
+    while (n > 2 * p.N + 16) {
+      float m = -INFINITY;
+#pragma unroll 1
+      for (int i = tid; i < n; i += kBeamThreads) m = fmaxf(m, __double2float_rd(list_t[cur][i]));
+      gmax[tid] = m;
+      if (tid == 0) sh_count[cur ^ 1] = 0;
+      __syncthreads();
+      float pivot;
+      if (p.N <= 32) {
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) {
-        const double t2 = __shfl_xor_sync(0xffffffffu, bt, off);
-        const unsigned int a2 = __shfl_xor_sync(0xffffffffu, ba, off);
-        if (beam_before(t2, a2, bt, ba)) {
-          bt = t2;
-          ba = a2;
+        for (int w = 0; w < kBeamThreads / 32; ++w) m = fmaxf(m, gmax[w * 32 + lane]);
+        pivot = warp_nth(m, p.N);
+      } else {
+        float4 v4;
+        v4.x = fmaxf(gmax[lane], gmax[lane + 128]);
+        v4.y = fmaxf(gmax[lane + 32], gmax[lane + 160]);
+        v4.z = fmaxf(gmax[lane + 64], gmax[lane + 192]);
+        v4.w = fmaxf(gmax[lane + 96], gmax[lane + 224]);
+        pivot = warp_nth4(v4, p.N);
+      }
+#pragma unroll 1
+      for (int i = tid; i < n; i += kBeamThreads) {
+        const double t = list_t[cur][i];
+        if (__double2float_rd(t) >= pivot) {
+          const int pos = atomicAdd(&sh_count[cur ^ 1], 1);
+          list_t[cur ^ 1][pos] = t;
+          list_a[cur ^ 1][pos] = list_a[cur][i];
         }
       }
       __syncthreads();
-      if (lane == 0) {
-        list_t[warp] = bt;
-        list_a[warp] = ba;
+      cur ^= 1;
+      if (sh_count[cur] * 4 > n * 3) {  // not much less: many equal totals
+        n = sh_count[cur];
+        break;
       }
-      __syncthreads();
-      for (int w = 0; w < kBeamThreads / 32; ++w)
-        if (beam_before(list_t[w], list_a[w], bt, ba)) {
-          bt = list_t[w];
-          ba = list_a[w];
-        }
-      if (tid == 0) put(i, bt, ba);  // n > N entries exist: every round finds one
-      lt = bt;
-      la = ba;
+      n = sh_count[cur];
     }
+    // ranks; those that make it go out, or to the front of the other list
+    const bool end = last == items;
+#pragma unroll 1
+    for (int i = tid; i < n; i += kBeamThreads) {
+      const double t = list_t[cur][i];
+      const unsigned int a = list_a[cur][i];
+      int rank = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) rank += beam_before(list_t[cur][j], list_a[cur][j], t, a);
+      if (rank >= p.N) continue;
+      if (end) {
+        p.out_scores[o + rank] = (float)t;
+        p.out_tokens[o + rank] = (long long)(a % (unsigned int)p.V);
+        p.out_parents[o + rank] = (long long)(a / (unsigned int)p.V);
+      } else {
+        list_t[cur ^ 1][rank] = t;
+        list_a[cur ^ 1][rank] = a;
+      }
+    }
+    have = min(n, p.N);
+    cur ^= 1;
   }
-  for (int i = found + tid; i < p.N; i += kBeamThreads) {
+  for (int i = have + tid; i < p.N; i += kBeamThreads) {
     p.out_scores[o + i] = -INFINITY;
     p.out_tokens[o + i] = -1;
     p.out_parents[o + i] = min(i, p.K - 1);

@@ -119,13 +119,23 @@ static int int4_launch_rows(const Int4Params& p, const Int4Plan& pl, int group, 
 // ---- beam step ----------------------------------------------------------------------------------
 static int beam_element_bytes(int dtype) { return dtype == FMMS_F32 ? 4 : 2; }
 
-static int beam_splits(int V, int dtype) {
-  const int es = beam_element_bytes(dtype), tile = kBeamThreads * kBeamVecs * (16 / es);
-  return (V + 16 / es - 1 + tile - 1) / tile;  // a row may start anywhere within 16 bytes
+// Vectors of a thread in a slice of a row, and slices of a row: as few slices as the list for their candidates allows,
+// but enough that the rows together make some four CTAs for each of the 148 SMs; not below four vectors, which the bound
+// is taken from.
+static void beam_slices(int rows, int V, int dtype, int* iters, int* splits) {
+  const long long per_iter = kBeamThreads * (16 / beam_element_bytes(dtype));
+  const long long all = (V + per_iter - 1) / per_iter;
+  long long want = (4 * 148 + rows - 1) / rows;
+  long long it = (all + want - 1) / want;
+  it = it < kBeamFirst ? kBeamFirst : it > kBeamMaxIters ? kBeamMaxIters : it;
+  *iters = (int)it;
+  *splits = (int)((all + it - 1) / it);
 }
 
 static size_t beam_workspace(int R, int K, int V, int N, int dtype) {
-  const size_t parts = (size_t)R * K * beam_splits(V, dtype);
+  int iters, splits;
+  beam_slices(R * K, V, dtype, &iters, &splits);
+  const size_t parts = (size_t)R * K * splits;
   return parts * N * 8 + parts * 8 + parts * 4;
 }
 
@@ -244,7 +254,7 @@ int fmms_beam_step(const void* logits, int dtype, long long stride_r, long long 
   p.K = K;
   p.V = V;
   p.N = N;
-  p.splits = beam_splits(V, dtype);
+  beam_slices(R * K, V, dtype, &p.iters, &p.splits);
   p.pad_token = pad_token;
   const size_t parts = (size_t)R * K * p.splits;
   p.keys = reinterpret_cast<unsigned long long*>(workspace);

@@ -92,9 +92,10 @@ def beam_search_step(
         finished = finished.contiguous()
         done = finished.data_ptr()
     step = BeamStep(
-        torch.empty((R, N), dtype=torch.float32, device=dev),
-        torch.empty((R, N), dtype=torch.int64, device=dev),
-        torch.empty((R, N), dtype=torch.int64, device=dev),
+        # empty_strided: the allocation with the least host time
+        torch.empty_strided((R, N), (N, 1), dtype=torch.float32, device=dev),
+        torch.empty_strided((R, N), (N, 1), dtype=torch.int64, device=dev),
+        torch.empty_strided((R, N), (N, 1), dtype=torch.int64, device=dev),
     )
     if R == 0:
         return step

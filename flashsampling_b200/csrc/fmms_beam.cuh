@@ -9,10 +9,11 @@
 //
 // The N largest of a set are found through a bound: split the set into G >= N groups; the N-th largest of the groups'
 // maxima cannot exceed the N-th largest element.  What reaches the bound is N elements and, with random order, few more
-// (G = 32: 9.2 of 8, 22 of 16).  A slice takes a first bound from its first quarter and notes the vectors with an element
-// that reaches it; the final bound, from the whole slice, picks the elements, which are counted against each other for
-// their ranks.  Where the first bound leaves too many vectors (tokens masked there, logits that rise), all are looked at
-// again; where the final one leaves too many elements (many equal logits), the N largest are taken one after the other.
+// (G = 32: 9.2 of 8, 22 of 16).  A slice takes its bound from its first vectors and keeps the vectors with an element that
+// reaches it (from a quarter of the slice: four times as many); their elements are counted against each other for their
+// ranks.  Where that is more than the lists hold (tokens masked in the first vectors, logits that rise), the slice is looked
+// at again with a bound from all of it, and where even that leaves too many (equal logits), the N largest are taken one
+// after the other.
 //
 // Two beams' candidates may lie arbitrarily close, and their order is an integer output, so sums and totals are formed
 // to more than 32 bits: exponentials carry the rounding of their argument along, slices join in fp64, and totals are
@@ -21,6 +22,7 @@
 
 #include <cuda_fp16.h>
 
+#include <cfloat>
 #include <type_traits>
 
 #include "fmms_common.cuh"
@@ -30,11 +32,11 @@ namespace fmms {
 constexpr int kBeamThreads = 256;
 constexpr int kBeamMaxN = 64;       // candidates
 constexpr int kBeamMaxK = 64;       // beams
-constexpr int kBeamRing = 6;        // 16-byte vectors a thread has in flight or in hand
+constexpr int kBeamRing = 3;        // pairs of 16-byte vectors a thread has in flight or in hand
 constexpr int kBeamFirst = 4;       // vectors of a thread that the bound is taken from
-constexpr int kBeamMaxIters = 16;   // vectors of a thread in a slice
-constexpr int kBeamVecCap = 768;    // vectors of a slice with an element that reaches the first bound
-constexpr int kBeamListCap = 512;   // elements of a slice that reach the final bound
+constexpr int kBeamMaxIters = 16;   // vectors of a thread in a slice (even)
+constexpr int kBeamVecCap = 448;    // vectors of a slice with an element that reaches the bound
+constexpr int kBeamListCap = 512;   // elements of a slice that reach the bound
 constexpr int kBeamItems = 1024;    // entries that the merge holds at a time
 constexpr int kBeamMergeCap = kBeamItems + kBeamMaxN;
 
@@ -117,50 +119,56 @@ __device__ __forceinline__ double beam_log(double x) {
   return y + fma(x, beam_exp(-y), -1.);
 }
 
-// The n-th largest of 32 values, one per lane (equal ones in the order of the lanes).
+// The n-th largest of 32 values, one per lane: sorted by a bitonic network, descending over the lanes.
 __device__ __forceinline__ float warp_nth(float v, int n) {
   const int lane = threadIdx.x & 31;
-  int rank = 0;
-#pragma unroll 8
-  for (int i = 0; i < 32; ++i) {
-    const float o = __shfl_sync(0xffffffffu, v, i);
-    rank += o > v || (o == v && i < lane);
-  }
-  return __shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, rank == n - 1)) - 1);
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int j = size >> 1; j > 0; j >>= 1) {
+      const float o = __shfl_xor_sync(0xffffffffu, v, j);
+      v = ((lane & j) == 0) == ((lane & size) == 0) ? fmaxf(v, o) : fminf(v, o);
+    }
+  return __shfl_sync(0xffffffffu, v, n - 1);
 }
 
 // The same of 128 values, four per lane.
 __device__ __noinline__ float warp_nth4(float4 v4, int n) {
   const int lane = threadIdx.x & 31;
-  const float v[4] = {v4.x, v4.y, v4.z, v4.w};
-  int rank[4] = {0, 0, 0, 0};
-#pragma unroll 1
-  for (int i = 0; i < 32; ++i)
+  float v[4] = {v4.x, v4.y, v4.z, v4.w};  // value 32 r + lane
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float o = __shfl_sync(0xffffffffu, v[q], i);
+  for (int size = 2; size <= 128; size <<= 1)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) rank[r] += o > v[r] || (o == v[r] && q * 32 + i < r * 32 + lane);
+    for (int j = size >> 1; j > 0; j >>= 1) {
+      float o[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = j < 32 ? __shfl_xor_sync(0xffffffffu, v[r], j) : v[r ^ (j >> 5)];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int e = 32 * r + lane;
+        v[r] = ((e & j) == 0) == ((e & size) == 0) ? fmaxf(v[r], o[r]) : fminf(v[r], o[r]);
+      }
     }
-  float found = -INFINITY;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const unsigned b = __ballot_sync(0xffffffffu, rank[r] == n - 1);
-    if (b) found = __shfl_sync(0xffffffffu, v[r], __ffs(b) - 1);
-  }
-  return found;
+  const int r = (n - 1) >> 5;
+  return __shfl_sync(0xffffffffu, r == 0 ? v[0] : r == 1 ? v[1] : r == 2 ? v[2] : v[3], (n - 1) & 31);
+}
+
+__device__ __forceinline__ void copy_vector(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamParams p) {
   constexpr int VE = 16 / sizeof(T);
-  __shared__ __align__(16) uint4 ring[kBeamRing][kBeamThreads];
+  __shared__ __align__(16) uint4 ring[kBeamRing][2][kBeamThreads];
   __shared__ __align__(16) float gmax[128];
   __shared__ float sh_pivot;
   __shared__ int sh_vecs, sh_count;
+  __shared__ __align__(16) uint4 vec_data[kBeamVecCap];
   __shared__ int vec_list[kBeamVecCap];
   __shared__ unsigned long long list[kBeamListCap];
   __shared__ double wsum[kBeamThreads / 32], wsum_up[kBeamThreads / 32];
+  __shared__ float wmax[kBeamThreads / 32];
   __shared__ unsigned long long wbest[kBeamThreads / 32];
   griddep_launch_dependents();
   const int row = blockIdx.y, split = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -174,13 +182,13 @@ __global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamPa
   const int singles = (split == 0 ? lead : 0) + (split == p.splits - 1 ? p.V - tail : 0);
   const T* xv = x + lead;
 
-  auto fetch = [&](int v, int slot) {  // vector v of the row, for this thread
-    if (v < v_end)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&ring[slot][tid])), "l"(xv + (size_t)v * VE) : "memory");
+  auto fetch = [&](int v, int slot) {  // vectors v and v + 256 of the row, for this thread
+    if (v < v_end) copy_vector(&ring[slot][0][tid], xv + (size_t)v * VE);
+    if (v + kBeamThreads < v_end) copy_vector(&ring[slot][1][tid], xv + (size_t)(v + kBeamThreads) * VE);
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int i = 0; i < kBeamRing - 1; ++i) fetch(v_begin + i * kBeamThreads + tid, i);
+  for (int i = 0; i < kBeamRing - 1; ++i) fetch(v_begin + 2 * i * kBeamThreads + tid, i);
   float single = -INFINITY;
   int single_at = 0;
   if (tid < singles) {  // at most 2 (VE - 1) threads
@@ -191,11 +199,11 @@ __global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamPa
   if (tid == 0) sh_vecs = sh_count = 0;
 
   // bound and first reference of the exponentials from the first vectors (fmaxf drops NaN)
-  asm volatile("cp.async.wait_group %0;" ::"n"(kBeamRing - 1 - kBeamFirst) : "memory");
+  asm volatile("cp.async.wait_group %0;" ::"n"(kBeamRing - 1 - kBeamFirst / 2) : "memory");
   float m = single;
-#pragma unroll 1
+#pragma unroll
   for (int i = 0; i < kBeamFirst; ++i)
-    if (v_begin + i * kBeamThreads + tid < v_end) m = fmaxf(m, beam_vec_max<T>(ring[i][tid]));
+    if (v_begin + i * kBeamThreads + tid < v_end) m = fmaxf(m, beam_vec_max<T>(ring[i / 2][i % 2][tid]));
   // The N-th largest of 32 groups' maxima (8 lanes each; up to 32 candidates), or of 128 (2 lanes): into sh_pivot; the
   // largest: returned.
   const bool wide = p.N <= 32;
@@ -258,36 +266,46 @@ __global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamPa
   if (tid < singles) {
     add(make_float2(single, -INFINITY));  // not above ref
   }
+  // below this a vector neither raises the reference (which the bound never exceeds) nor is noted; nothing is at -inf
+  const float quiet = fmaxf(pivot, -FLT_MAX);
+  auto note = [&](int v, const uint4& u) {
+    const int pos = atomicAdd(&sh_vecs, 1);
+    if (pos < kBeamVecCap) {
+      vec_list[pos] = v;
+      vec_data[pos] = u;
+    }
+  };
   const uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -inf
-  int slot = 0, next = kBeamRing - 1;
 #pragma unroll 1
-  for (int i = 0, v = v_begin + tid; i < p.iters; ++i, v += kBeamThreads) {
+  for (int i = 0, v = v_begin + tid; i < p.iters / 2; ++i, v += 2 * kBeamThreads) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kBeamRing - 2) : "memory");
-    uint4 u = make_uint4(kNone, kNone, kNone, kNone);
-    if (v < v_end) u = ring[slot][tid];
-    fetch(v + (kBeamRing - 1) * kBeamThreads, next);
-    const float vm = beam_vec_max<T>(u);
+    const int slot = i % kBeamRing;
+    uint4 u0 = make_uint4(kNone, kNone, kNone, kNone), u1 = u0;
+    if (v < v_end) u0 = ring[slot][0][tid];
+    if (v + kBeamThreads < v_end) u1 = ring[slot][1][tid];
+    fetch(v + 2 * (kBeamRing - 1) * kBeamThreads, (i + kBeamRing - 1) % kBeamRing);
+    const float vm0 = beam_vec_max<T>(u0), vm1 = beam_vec_max<T>(u1), vm = fmaxf(vm0, vm1);
     m = fmaxf(m, vm);
     // rare, and left together: the exponentials below are the warp's again
-    if (vm > ref) raise(vm);
-    if (vm >= pivot && vm > -INFINITY) {
-      const int pos = atomicAdd(&sh_vecs, 1);
-      if (pos < kBeamVecCap) vec_list[pos] = v;
+    if (vm >= quiet) {
+      if (vm > ref) raise(vm);
+      if (vm0 >= quiet) note(v, u0);
+      if (vm1 >= quiet) note(v + kBeamThreads, u1);
     }
     __syncwarp();
 #pragma unroll
-    for (int q = 0; q < VE / 2; ++q) add(beam_get<T>(u, q));
-    if (++slot == kBeamRing) slot = 0;
-    if (++next == kBeamRing) next = 0;
+    for (int q = 0; q < VE / 2; ++q) add(beam_get<T>(u0, q));
+#pragma unroll
+    for (int q = 0; q < VE / 2; ++q) add(beam_get<T>(u1, q));
   }
   const double mine = sum_now();
-  float top = ref0;
-  if (p.iters > kBeamFirst) {  // else the first bound is that of the whole slice
-    top = bound(m);
-    pivot = sh_pivot;
-  } else {
-    __syncthreads();  // the noted vectors are complete
-  }
+  float top = m;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  if (lane == 0) wmax[warp] = top;
+  __syncthreads();  // also: the noted vectors are complete
+#pragma unroll
+  for (int w = 0; w < kBeamThreads / 32; ++w) top = fmaxf(top, wmax[w]);
   // threads whose reference is still the first one add up in its units, the others in those of the slice's maximum
   double sum = ref == ref0 ? mine : 0., sum_up = 0.;
   if (ref != ref0 && mine > 0.) sum_up = mine * beam_exp((double)ref - (double)top);
@@ -301,23 +319,23 @@ __global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamPa
     wsum[warp] = sum;
     wsum_up[warp] = sum_up;
   }
-  // the elements that reach the bound: of the noted vectors, or of all where too many were noted
+  // the elements that reach the bound
   auto offer = [&](float v, int at) {
     if (v >= pivot && v > -INFINITY) {
       const int pos = atomicAdd(&sh_count, 1);
       if (pos < kBeamListCap) list[pos] = cand_key(v + 0.f, at);  // + 0.f: -0 counts as 0
     }
   };
-  const bool noted = sh_vecs <= kBeamVecCap;
-  const int look = (noted ? sh_vecs : v_end - v_begin) * VE;
+  const int vecs_noted = sh_vecs;
+  if (vecs_noted <= kBeamVecCap) {
 #pragma unroll 1
-  for (int i = tid; i < look; i += kBeamThreads) {
-    const int at = lead + (noted ? vec_list[i / VE] : v_begin + i / VE) * VE + i % VE;
-    offer((float)x[at], at);
+    for (int i = tid; i < vecs_noted * VE; i += kBeamThreads)
+      offer((float)reinterpret_cast<const T*>(vec_data)[i], lead + vec_list[i / VE] * VE + i % VE);
+    if (tid < singles) offer(single, single_at);
   }
-  if (tid < singles) offer(single, single_at);
   __syncthreads();
-  const int n = sh_count;
+  int n = sh_count;
+  const int from = split == 0 ? 0 : lead + v_begin * VE, to = split == p.splits - 1 ? p.V : lead + v_end * VE;
   const size_t part = (size_t)row * p.splits + split;
   unsigned long long* out = p.keys + part * p.N;
   if (tid == kBeamThreads - 1) {  // the last warp: the first ones rank the list
@@ -329,7 +347,55 @@ __global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamPa
     p.sums[part] = (ref0 == top || all == 0. ? all : all * beam_exp((double)ref0 - (double)top)) + up;
     p.maxima[part] = top;
   }
+  if (vecs_noted > kBeamVecCap || n > kBeamListCap) {
+    bound(m);  // of the whole slice now
+    pivot = sh_pivot;
+    if (tid == 0) sh_count = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = from + tid; i < to; i += kBeamThreads) offer((float)x[i], i);
+    __syncthreads();
+    n = sh_count;
+  }
   if (n <= kBeamListCap) {
+    if (n > 64 && n <= 256 && p.N <= 32) {
+      // The first warp alone: a bound from 32 groups of the list, what reaches it moved to the front, and if that is one
+      // element per lane at most, sorted.
+      if (warp != 0) return;
+      float v = -INFINITY;
+      for (int i = lane; i < n; i += 32) v = fmaxf(v, float_key_decode((uint32_t)(list[i] >> 32)));
+      const float least = warp_nth(v, p.N);
+      int kept = 0;
+      for (int i0 = 0; i0 < n; i0 += 32) {
+        const unsigned long long key = i0 + lane < n ? list[i0 + lane] : 0ull;
+        const bool in = key != 0ull && float_key_decode((uint32_t)(key >> 32)) >= least;
+        const unsigned b = __ballot_sync(0xffffffffu, in);
+        if (in) list[kept + __popc(b & ((1u << lane) - 1u))] = key;  // at or before where it was read
+        kept += __popc(b);
+        __syncwarp();
+      }
+      unsigned long long key = lane < kept ? list[lane] : 0ull;
+      if (kept <= 32) {
+#pragma unroll
+        for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+          for (int j = size >> 1; j > 0; j >>= 1) {
+            const unsigned long long o = __shfl_xor_sync(0xffffffffu, key, j);
+            key = ((lane & j) == 0) == ((lane & size) == 0) ? max(key, o) : min(key, o);
+          }
+        if (lane < p.N) out[lane] = key;
+        return;
+      }
+      n = kept;
+      for (int i = lane; i < n; i += 32) {
+        key = list[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) rank += list[j] > key;
+        if (rank < p.N) out[rank] = key;
+      }
+      return;  // n > 32 >= N: every place is taken
+    }
     for (int i = tid; i < n; i += kBeamThreads) {
       const unsigned long long key = list[i];
       int rank = 0;
@@ -341,7 +407,6 @@ __global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamPa
     return;
   }
   // many elements at the bound: one maximum after the other (keys differ, each is below the last), read again
-  const int from = split == 0 ? 0 : lead + v_begin * VE, to = split == p.splits - 1 ? p.V : lead + v_end * VE;
   unsigned long long last = ~0ull;
   for (int r = 0; r < p.N; ++r) {
     unsigned long long best = 0ull;

@@ -128,6 +128,7 @@ static void beam_slices(int rows, int V, int dtype, int* iters, int* splits) {
   long long want = (4 * 148 + rows - 1) / rows;
   long long it = (all + want - 1) / want;
   it = it < kBeamFirst ? kBeamFirst : it > kBeamMaxIters ? kBeamMaxIters : it;
+  it += it & 1;
   *iters = (int)it;
   *splits = (int)((all + it - 1) / it);
 }
@@ -320,7 +321,7 @@ int fmms_reorder_beams(const fmms_beam_state_t* states, int n_states, const void
         d.vec = vec;
         const long long cols = s.seg_bytes / vec, unit = kReorderThreads * U, outers = (long long)s.outer[0] * s.outer[1];
         if (nr * ((cols + unit - 1) / unit) >= (1ll << 31)) return FMMS_ERR_UNSUPPORTED;
-        const long long units = cols >= unit / 2 ? outers * nr * ((cols + unit - 1) / unit) : (outers * nr * cols + unit - 1) / unit;
+        const long long units = cols >= unit / 2 ? outers * nr * ((cols + unit - 1) / unit) : (outers * nr * cols + kReorderThreads - 1) / kReorderThreads;
         if (units > most) most = units;
       }
       // CTAs: enough to fill the GPU eight times over all tensors together, not more than a tensor has work for

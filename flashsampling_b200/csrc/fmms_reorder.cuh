@@ -64,27 +64,13 @@ __device__ __forceinline__ void reorder_columns(const ReorderParams& p, const Re
   const long long cols = s.seg_bytes / VEC;
   const long long outers = (long long)s.outer[0] * s.outer[1];
 
-  auto move = [&](uint8_t* const (&at)[U], const int (&req)[U]) {  // req < 0: nothing to do
-    V v[U][KM];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < KM; ++j)
-        if (req[u] >= 0 && j < p.K) {
-          const int par = reorder_parent(p, req[u], j);
-          if (par != j) v[u][j] = *reinterpret_cast<const V*>(at[u] + par * s.beam_stride);
-        }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < KM; ++j)
-        if (req[u] >= 0 && j < p.K && reorder_parent(p, req[u], j) != j) *reinterpret_cast<V*>(at[u] + j * s.beam_stride) = v[u][j];
-  };
-
   if (cols >= kUnit / 2) {
-    // long segments: a unit is kUnit columns of one (outer index, request); prefix[r]: live units of the requests below r
+    // Long segments: a unit is kUnit columns of one (outer index, request), so that the parents are read once per unit.
+    // prefix[r]: live units of the requests below r.
     const int per_outer = prefix[p.R];
-    for (long long unit = blockIdx.x; unit < outers * per_outer; unit += gridDim.x) {
+    const long long units = outers * per_outer;
+#pragma unroll 1
+    for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
       const long long o = unit / per_outer;
       const int i = (int)(unit - o * per_outer);
       int lo = 0, hi = p.R - 1;  // the last r with prefix[r] <= i
@@ -96,41 +82,51 @@ __device__ __forceinline__ void reorder_columns(const ReorderParams& p, const Re
       long long live = cols;
       if (p.lengths && s.step_bytes) live = min(cols, max(0, p.lengths[r]) * (s.step_bytes / VEC));
       const long long o0 = o / s.outer[1], o1 = o - o0 * s.outer[1];
-      uint8_t* seg = s.data + o0 * s.outer_stride[0] + o1 * s.outer_stride[1] + (long long)r * p.K * s.beam_stride;
-      uint8_t* at[U];
-      int req[U];
+      const long long col = (long long)(i - prefix[r]) * kUnit + tid;
+      uint8_t* at = s.data + o0 * s.outer_stride[0] + o1 * s.outer_stride[1] + (long long)r * p.K * s.beam_stride + col * VEC;
+      int par[KM];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const long long col = (long long)(i - prefix[r]) * kUnit + u * kReorderThreads + tid;
-        at[u] = seg + col * VEC;
-        req[u] = col < live ? r : -1;
-      }
-      move(at, req);
+      for (int j = 0; j < KM; ++j) par[j] = j < p.K ? reorder_parent(p, r, j) : j;
+      V v[U][KM];
+#pragma unroll
+      for (int j = 0; j < KM; ++j)
+        if (par[j] != j) {
+          const uint8_t* src = at + par[j] * s.beam_stride;
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (col + u * kReorderThreads < live) v[u][j] = *reinterpret_cast<const V*>(src + u * kReorderThreads * VEC);
+        }
+#pragma unroll
+      for (int j = 0; j < KM; ++j)
+        if (par[j] != j) {
+          uint8_t* dst = at + j * s.beam_stride;
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (col + u * kReorderThreads < live) *reinterpret_cast<V*>(dst + u * kReorderThreads * VEC) = v[u][j];
+        }
     }
     return;
   }
-  // short segments: the columns of all (outer index, request) one after the other
+  // Short segments: the columns of all (outer index, request) one after the other.
   const long long total = outers * p.R * cols;
-  for (long long base = (long long)blockIdx.x * kUnit; base < total; base += (long long)gridDim.x * kUnit) {
-    uint8_t* at[U];
-    int req[U];
+#pragma unroll 1
+  for (long long x = (long long)blockIdx.x * kReorderThreads + tid; x < total; x += (long long)gridDim.x * kReorderThreads) {
+    const long long seg = x / cols, col = x - seg * cols;
+    const long long o = seg / p.R;
+    const int r = (int)(seg - o * p.R);
+    if (p.lengths && s.step_bytes && col >= max(0, p.lengths[r]) * (s.step_bytes / VEC)) continue;
+    const long long o0 = o / s.outer[1], o1 = o - o0 * s.outer[1];
+    uint8_t* at = s.data + o0 * s.outer_stride[0] + o1 * s.outer_stride[1] + (long long)r * p.K * s.beam_stride + col * VEC;
+    int par[KM];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long long x = base + u * kReorderThreads + tid;
-      req[u] = -1;
-      at[u] = s.data;
-      if (x < total) {
-        const long long seg = x / cols, col = x - seg * cols;
-        const long long o = seg / p.R;
-        const int r = (int)(seg - o * p.R);
-        const long long o0 = o / s.outer[1], o1 = o - o0 * s.outer[1];
-        long long live = cols;
-        if (p.lengths && s.step_bytes) live = min(cols, max(0, p.lengths[r]) * (s.step_bytes / VEC));
-        if (col < live) req[u] = r;
-        at[u] = s.data + o0 * s.outer_stride[0] + o1 * s.outer_stride[1] + (long long)r * p.K * s.beam_stride + col * VEC;
-      }
-    }
-    move(at, req);
+    for (int j = 0; j < KM; ++j) par[j] = j < p.K ? reorder_parent(p, r, j) : j;
+    V v[KM];
+#pragma unroll
+    for (int j = 0; j < KM; ++j)
+      if (par[j] != j) v[j] = *reinterpret_cast<const V*>(at + par[j] * s.beam_stride);
+#pragma unroll
+    for (int j = 0; j < KM; ++j)
+      if (par[j] != j) *reinterpret_cast<V*>(at + j * s.beam_stride) = v[j];
   }
 }
 

@@ -82,9 +82,9 @@ static size_t int4_workspace(const Int4Plan& pl, int V, int B) {
   return blocks * (tiles + 1) * pl.nt * 512;
 }
 
-template <int NT, int GR, bool ZP>
+template <int NT, int GR, bool ZP, int W>
 static int int4_launch(const Int4Params& p, const Int4Plan& pl, int dev, int num_sms, cudaStream_t stream) {
-  auto* kernel = int4_linear_kernel<NT, GR, ZP>;
+  auto* kernel = int4_linear_kernel<NT, GR, ZP, W>;
   static std::atomic<bool> ready[kDecodeMaxDevices];
   if (!ready[dev].load(std::memory_order_acquire)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kInt4SmemLimit) != cudaSuccess) {
@@ -94,25 +94,25 @@ static int int4_launch(const Int4Params& p, const Int4Plan& pl, int dev, int num
     ready[dev].store(true, std::memory_order_release);
   }
   const dim3 grid((unsigned)min(p.tiles, num_sms), (unsigned)((p.B + NT * 8 - 1) / (NT * 8)));
-  kernel<<<grid, pl.warps * 32, pl.smem, stream>>>(p);
+  kernel<<<grid, W * 32, pl.smem, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
 
-template <int NT, bool ZP>
-static int int4_launch_group(const Int4Params& p, const Int4Plan& pl, int group, int dev, int num_sms, cudaStream_t stream) {
-  switch (group) {
-    case 32: return int4_launch<NT, 32, ZP>(p, pl, dev, num_sms, stream);
-    case 64: return int4_launch<NT, 64, ZP>(p, pl, dev, num_sms, stream);
-    default: return int4_launch<NT, 128, ZP>(p, pl, dev, num_sms, stream);
+template <int GR, bool ZP>
+static int int4_launch_rows(const Int4Params& p, const Int4Plan& pl, int dev, int num_sms, cudaStream_t stream) {
+  switch (pl.nt) {
+    case 1: return int4_launch<1, GR, ZP, 16>(p, pl, dev, num_sms, stream);
+    case 2: return pl.warps == 8 ? int4_launch<2, GR, ZP, 8>(p, pl, dev, num_sms, stream) : int4_launch<2, GR, ZP, 16>(p, pl, dev, num_sms, stream);
+    default: return int4_launch<4, GR, ZP, 8>(p, pl, dev, num_sms, stream);
   }
 }
 
 template <bool ZP>
-static int int4_launch_rows(const Int4Params& p, const Int4Plan& pl, int group, int dev, int num_sms, cudaStream_t stream) {
-  switch (pl.nt) {
-    case 1: return int4_launch_group<1, ZP>(p, pl, group, dev, num_sms, stream);
-    case 2: return int4_launch_group<2, ZP>(p, pl, group, dev, num_sms, stream);
-    default: return int4_launch_group<4, ZP>(p, pl, group, dev, num_sms, stream);
+static int int4_launch_group(const Int4Params& p, const Int4Plan& pl, int group, int dev, int num_sms, cudaStream_t stream) {
+  switch (group) {
+    case 32: return int4_launch_rows<32, ZP>(p, pl, dev, num_sms, stream);
+    case 64: return int4_launch_rows<64, ZP>(p, pl, dev, num_sms, stream);
+    default: return int4_launch_rows<128, ZP>(p, pl, dev, num_sms, stream);
   }
 }
 
@@ -222,7 +222,7 @@ int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void*
   p.ring_off = pl.ring_off;
   p.piece_off = pl.piece_off;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return zeros ? int4_launch_rows<true>(p, pl, group, dev, num_sms, s) : int4_launch_rows<false>(p, pl, group, dev, num_sms, s);
+  return zeros ? int4_launch_group<true>(p, pl, group, dev, num_sms, s) : int4_launch_group<false>(p, pl, group, dev, num_sms, s);
 }
 
 int fmms_query_beam_workspace(int R, int K, int V, int N, int dtype, size_t* bytes) {

@@ -111,9 +111,9 @@ __device__ __forceinline__ void int4_store(const Int4Params& p, int b, int v, fl
     reinterpret_cast<float*>(p.out)[at] = y;
 }
 
-// NT: blocks of eight rows of x; GR: columns of a group, at most 128; ZP: zero points given.
-template <int NT, int GR, bool ZP>
-__global__ void __launch_bounds__(NT == 4 ? 256 : 512, 1) int4_linear_kernel(const Int4Params p) {
+// NT: blocks of eight rows of x; GR: columns of a group, at most 128; ZP: zero points given; W: warps.
+template <int NT, int GR, bool ZP, int W>
+__global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kChunks = kInt4Unit / kInt4Chunk, kGroups = int4_unit_groups(GR);  // of a unit
   constexpr int kStage = int4_stage_bytes(GR), S = kInt4Stages;
@@ -121,9 +121,9 @@ __global__ void __launch_bounds__(NT == 4 ? 256 : 512, 1) int4_linear_kernel(con
   constexpr int kScaleCopy = kGroups == 4 ? 8 : 4;                    // bytes a lane copies of the scales
   constexpr int kScaleLanes = kGroups * 32 / kScaleCopy;              // lanes of one tile
   constexpr int kZeroLanes = kGroups * 4;
-  __shared__ unsigned int row_max[NT * 8], warp_max[16 * NT * 8];
-  __shared__ int part[18];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, W = blockDim.x >> 5;
+  __shared__ unsigned int warp_max[W * NT * 8];
+  __shared__ int row_exp[NT * 8];  // x went in times two to this
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   const int b0 = blockIdx.y * NT * 8, nb = min(NT * 8, p.B - b0);
 
@@ -134,13 +134,28 @@ __global__ void __launch_bounds__(NT == 4 ? 256 : 512, 1) int4_linear_kernel(con
   const uint8_t* ring = smem + p.ring_off + warp * (S * kStage);
   const uint32_t ring_at = smem_u32(ring);
 
+  // x: a thread has one row and one t, and 8 of every 32 columns: the 16 bytes of one lane's operands.  The first loads go
+  // out before anything else, the ring's behind them.
+  const int stride = (W * 8) >> p.log_rows, first_block = (tid >> 2) >> p.log_rows;
+  const int row = (tid >> 2) & ((1 << p.log_rows) - 1);
+  constexpr int kAhead = 4;  // loads in flight
+  uint4 raw[kAhead];
+  auto load_blocks = [&](int k_begin, int blocks, int from) {  // blocks of 32 columns; zero from p.D on
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int blk = from + i * stride;
+      raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < nb && blk < blocks && k_begin + blk * 32 < p.D) raw[i] = int4_load_x(p, b0 + row, k_begin + blk * 32 + t * 2);
+    }
+  };
+  load_blocks(0, p.units * (kInt4Unit / 32), first_block);
+
   // this CTA's tiles in pairs, and the warps' parts of them; position = pair * units + unit
-  const int t_begin = (int)((unsigned long long)p.tiles * blockIdx.x / gridDim.x);
-  const int t_end = (int)((unsigned long long)p.tiles * (blockIdx.x + 1) / gridDim.x);
-  const int pairs = (t_end - t_begin + 1) / 2;
-  if (tid <= W) part[tid] = (int)((long long)pairs * p.units * tid / W);
-  __syncthreads();
-  const int begin = part[warp], end = part[warp + 1];
+  const int t_each = p.tiles / (int)gridDim.x, t_rest = p.tiles - t_each * (int)gridDim.x;
+  const int t_begin = t_each * (int)blockIdx.x + min((int)blockIdx.x, t_rest), t_end = t_begin + t_each + ((int)blockIdx.x < t_rest);
+  const int span = (t_end - t_begin + 1) / 2 * p.units, s_each = span / W, s_rest = span - s_each * W;
+  auto part = [&](int w) { return s_each * w + min(w, s_rest); };
+  const int begin = part(warp), end = part(warp + 1);
   const int p_first = begin / p.units, p_last = (end - 1) / p.units;
   // the units of pair `pr` in `phase` that belong to this warp: from lo to before hi
   auto unit_range = [&](int phase, int pr, int& lo, int& hi) {
@@ -209,12 +224,6 @@ __global__ void __launch_bounds__(NT == 4 ? 256 : 512, 1) int4_linear_kernel(con
   for (int i = 0; i < S - 1; ++i) fetch();
 
   auto pow2 = [](int e) { return __uint_as_float((uint32_t)(e + 127) << 23); };
-  // exponent of the power of two that puts the row's maximum into [2^14, 2^15); clamped to what fp32 can hold
-  auto row_exponent = [&](int b) {
-    const int e = (int)(row_max[b] >> 23) - 127;
-    return row_max[b] == 0u ? 0 : min(14 - e, 120);
-  };
-
   float tot[2][NT][4];
   auto clear = [&] {
 #pragma unroll
@@ -240,61 +249,57 @@ __global__ void __launch_bounds__(NT == 4 ? 256 : 512, 1) int4_linear_kernel(con
   int slot = 0;
 
   for (int phase = 0; phase < p.phases; ++phase) {
-    // x: maximum of each row, then fp16 operands in the order the products read them, and the sums over the groups.
-    // A thread has one row and one t, and 8 of every 32 columns: the 16 bytes of one lane's operands.  Its first loads stay
-    // in registers from the maximum to the conversion.
-    const int k_begin = phase * p.units * kInt4Unit;
-    const int blocks = min(p.units, p.all_units - phase * p.units) * (kInt4Unit / 32);  // of 32 columns; zero from p.D on
-    const int stride = (W * 8) >> p.log_rows, first_block = (tid >> 2) >> p.log_rows;
-    const int row = (tid >> 2) & ((1 << p.log_rows) - 1);
-    constexpr int kAhead = 4;  // loads in flight
-    auto load_blocks = [&](int from, uint4 (&raw)[kAhead]) {
+    // x as it is into the places of its operands, with the maximum of each row on the way; then, each thread what it
+    // wrote itself, in fp16, and the sums over the groups
+    const int k_begin = phase * p.units * kInt4Unit, blocks = min(p.units, p.all_units - phase * p.units) * (kInt4Unit / 32);
+    uint4* const mine = xfrag + (row >> 3) * 32 + (row & 7) * 4 + t;
+    if (phase > 0) {
+      load_blocks(k_begin, blocks, first_block);
+      __syncthreads();  // the phase before has been read
+    }
+    uint32_t m = 0u;  // magnitudes of bf16 compare like integers
+#pragma unroll 1
+    for (int from = first_block; from < blocks; from += kAhead * stride) {
+      if (from != first_block) load_blocks(k_begin, blocks, from);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int blk = from + i * stride;
-        raw[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (row < nb && blk < blocks && k_begin + blk * 32 < p.D) raw[i] = int4_load_x(p, b0 + row, k_begin + blk * 32 + t * 2);
+        if (row < nb && blk < blocks) mine[blk * (NT * 32)] = raw[i];
+        m = __vmaxu2(m, __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu), __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu)));
       }
-    };
+    }
+    // the power of two that puts the row's maximum into [2^14, 2^15), clamped to what fp32 can hold; fp16 goes in as it is
     int exponent = 0;
-    if (p.x_bf16) {  // fp16 goes in as it is
-      uint32_t m = 0u;  // magnitudes of bf16 compare like integers
-#pragma unroll 1
-      for (int from = first_block; from < blocks; from += kAhead * stride) {
-        uint4 raw[kAhead];
-        load_blocks(from, raw);
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-          m = __vmaxu2(m, __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu), __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu)));
-      }
+    if (p.x_bf16) {
       m = max(m & 0xffffu, m >> 16);
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1)  // lanes of the same row
         if (off < 4 || off >= (4 << p.log_rows)) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
-      if (lane < (4 << p.log_rows) && t == 0 && row < nb) warp_max[warp * (NT * 8) + row] = m << 16;
-      __syncthreads();  // also: the phase before has been read
-      if (tid < nb) {
-        m = 0u;
-        // warps hold max(1, rows / 8) rows each: those of this one come round every so many warps
-        const int every = p.log_rows > 3 ? 1 << (p.log_rows - 3) : 1;
-        for (int w = (tid >> 3) & (every - 1); w < W; w += every) m = max(m, warp_max[w * (NT * 8) + tid]);
-        row_max[tid] = m;
-      }
+      if (lane < (4 << p.log_rows) && t == 0) warp_max[warp * (NT * 8) + row] = m;
       __syncthreads();
-      if (row < nb) exponent = row_exponent(row);
-    } else {
-      __syncthreads();
+      m = 0u;
+      // a warp has eight rows or all of them: this thread's row is in every `every`-th warp
+      const int every = p.log_rows > 3 ? 1 << (p.log_rows - 3) : 1;
+#pragma unroll 4
+      for (int w = (row >> 3) & (every - 1); w < W; w += every) m = max(m, warp_max[w * (NT * 8) + row]);
+      if (m != 0u) exponent = min(14 - ((int)(m >> 7) - 127), 120);
     }
+    if (first_block == 0 && t == 0 && row < nb) row_exp[row] = exponent;
     const float up = pow2(exponent);
+    constexpr int kConvert = 4;
 #pragma unroll 1
-    for (int from = first_block; from < blocks; from += kAhead * stride) {
-      uint4 raw[kAhead];
-      load_blocks(from, raw);
+    for (int from = first_block; from < blocks; from += kConvert * stride) {
+      uint4 x4[kConvert];
+      float s[kConvert];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int blk = from + i * stride;
-        uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-        float s = 0.f;
+      for (int i = 0; i < kConvert; ++i) {
+        x4[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < nb && from + i * stride < blocks) x4[i] = mine[(from + i * stride) * (NT * 32)];
+      }
+#pragma unroll
+      for (int i = 0; i < kConvert; ++i) {
+        uint32_t w[4] = {x4[i].x, x4[i].y, x4[i].z, x4[i].w};
+        s[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (p.x_bf16) {
@@ -302,15 +307,19 @@ __global__ void __launch_bounds__(NT == 4 ? 256 : 512, 1) int4_linear_kernel(con
             w[j] = *reinterpret_cast<const uint32_t*>(&h);
           }
           const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-          s += f.x + f.y;
+          s[i] += f.x + f.y;
         }
-        s += __shfl_xor_sync(0xfu << (lane & 28), s, 1);  // the four lanes of a row and block run together
-        s += __shfl_xor_sync(0xfu << (lane & 28), s, 2);
-        if (row < nb && blk < blocks) {
-          xfrag[(blk * NT + (row >> 3)) * 32 + (row & 7) * 4 + t] = make_uint4(w[0], w[1], w[2], w[3]);
-          // in units of the operands; without zero points times 8
-          if (t == 0) (GR == 32 ? xs : xs32)[blk * (NT * 8) + row] = s * (ZP ? -0x1p-24f : -0x1p-21f);
-        }
+        x4[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        s[i] += __shfl_xor_sync(0xfu << (lane & 28), s[i], 1);  // the four lanes of a row and block run together
+        s[i] += __shfl_xor_sync(0xfu << (lane & 28), s[i], 2);
+      }
+#pragma unroll
+      for (int i = 0; i < kConvert; ++i) {
+        const int blk = from + i * stride;
+        if (row >= nb || blk >= blocks) continue;
+        if (p.x_bf16) mine[blk * (NT * 32)] = x4[i];
+        // in units of the operands; without zero points times 8
+        if (t == 0) (GR == 32 ? xs : xs32)[blk * (NT * 8) + row] = s[i] * (ZP ? -0x1p-24f : -0x1p-21f);
       }
     }
     __syncthreads();
@@ -330,7 +339,7 @@ __global__ void __launch_bounds__(NT == 4 ? 256 : 512, 1) int4_linear_kernel(con
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int n = nt * 8 + t * 2 + i;
-        down[nt][i] = n < nb ? (p.x_bf16 ? pow2(-row_exponent(n)) : 1.f) : 0.f;
+        down[nt][i] = n < nb ? pow2(-row_exp[n]) : 0.f;
       }
 
     clear();
@@ -465,8 +474,9 @@ __global__ void __launch_bounds__(NT == 4 ? 256 : 512, 1) int4_linear_kernel(con
   if (begin < end) {
     const int pr = p_last, stop = (pr + 1) * p.units;
     if (begin <= pr * p.units && end < stop) {
-      for (int w = warp + 1; w < W && part[w] < stop; ++w) {
-        if (part[w] == part[w + 1]) continue;
+#pragma unroll 4
+      for (int w = warp + 1; w < W && part(w) < stop; ++w) {
+        if (part(w) == part(w + 1)) continue;
         const float* other = pieces + w * (2 * NT * 128) + lane;
 #pragma unroll
         for (int i = 0; i < 2 * NT * 4; ++i) tot[i / (NT * 4)][i / 4 % NT][i % 4] += other[i * 32];

@@ -165,7 +165,7 @@ SIGNATURES = {
             c_void_p, c_void_p, c_int, c_void_p,  # qweight, scales, scale_dtype, zeros
             c_int, c_int, c_int, c_int,  # V, D, group, B
             c_void_p, c_int, c_longlong,  # out, out_dtype, out_stride
-            c_void_p, c_size_t, c_void_p,  # workspace, workspace_bytes, stream
+            c_void_p, c_size_t, c_void_p, c_void_p,  # workspace, workspace_bytes, status_dev, stream
         ],
     ),
     "fmms_query_int4_workspace": (c_int, [c_int, c_int, c_int, c_int, ctypes.POINTER(c_size_t)]),

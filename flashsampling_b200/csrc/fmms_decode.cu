@@ -9,11 +9,13 @@
 #include "fmms_beam.cuh"
 #include "fmms_common.cuh"
 #include "fmms_int4.cuh"
+#include "fmms_int4_mma.cuh"
 #include "fmms_reorder.cuh"
 
 namespace fmms {
 
 constexpr int kDecodeMaxDevices = 16;
+constexpr int kInt4VectorRows = 8;  // rows of x up to which the products go to mma.sync
 constexpr int kInt4SmemLimit = 230000;  // of 232448 bytes a CTA may have; the rest: static shared memory
 
 static int decode_num_sms(int* dev_out, int* sms_out) {
@@ -31,6 +33,26 @@ static int decode_num_sms(int* dev_out, int* sms_out) {
   }
   *dev_out = dev;
   *sms_out = n;
+  return kOk;
+}
+
+// A kernel that may start while the one before it on the stream still runs (and waits for it where it needs it).
+template <typename... KArgs, typename... Args>
+static int launch_behind(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
+    cudaGetLastError();
+    return kErrCuda;
+  }
   return kOk;
 }
 
@@ -116,6 +138,71 @@ static int int4_launch_group(const Int4Params& p, const Int4Plan& pl, int group,
   }
 }
 
+// The tensor-core variant: rows of x in a pass, and the stages of x that fit beside the rings.
+struct Int4MmaPlan {
+  int n, passes, row_steps, x_stages, ring_off, scale_off, smem;
+};
+
+static void int4_mma_plan(Int4MmaPlan& pl, int D, int B, int group, bool zeros) {
+  const int gr = group < kInt4Unit ? group : kInt4Unit, most = int4_mma_max_n(gr);
+  pl.passes = (B + most - 1) / most;
+  pl.n = ((B + pl.passes - 1) / pl.passes + 15) / 16 * 16;
+  const int units = int4_step_units(gr, pl.n);
+  pl.row_steps = ((D + kInt4Unit - 1) / kInt4Unit + units - 1) / units;
+  const int weights = kInt4MmaWeightWarps * kInt4MmaRing * (units * 1024 + (zeros ? 64 : 0));
+  const int scales = kInt4MmaSumWarps * kInt4MmaScaleRing * int4_step_groups(gr, pl.n) * 64;
+  pl.x_stages = min(kInt4MmaMaxX, (kInt4SmemLimit - weights - scales) / int4_x_bytes(pl.n, gr));
+  pl.ring_off = pl.x_stages * int4_x_bytes(pl.n, gr);
+  pl.scale_off = pl.ring_off + weights;
+  pl.smem = pl.scale_off + scales;
+}
+
+// staged x, then the exponents of its rows
+static size_t int4_mma_workspace(int D, int B, int group) {
+  Int4MmaPlan pl;
+  int4_mma_plan(pl, D, B, group, true);
+  return (size_t)pl.passes * (pl.row_steps * (size_t)int4_x_bytes(pl.n, group < kInt4Unit ? group : kInt4Unit) + kInt4MmaPass * 4);
+}
+
+template <int NC, int GR, bool ZP>
+static int int4_mma_launch(const Int4MmaParams& p, const Int4MmaPlan& pl, int dev, int num_sms, uint8_t* staged, int* exponents, cudaStream_t stream) {
+  if constexpr (NC <= int4_mma_max_n(GR)) {
+    auto* kernel = int4_mma_kernel<NC, GR, ZP>;
+    static std::atomic<bool> ready[kDecodeMaxDevices];
+    if (!ready[dev].load(std::memory_order_acquire)) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kInt4SmemLimit) != cudaSuccess) {
+        cudaGetLastError();
+        return kErrCuda;
+      }
+      ready[dev].store(true, std::memory_order_release);
+    }
+    int4_stage_x_kernel<GR><<<p.base.B, 256, 0, stream>>>(p, staged, exponents);
+    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+    return launch_behind(kernel, dim3((unsigned)min(p.base.tiles, num_sms), (unsigned)pl.passes), kInt4MmaThreads, pl.smem, stream, p);
+  } else {
+    return kErrUnsupported;  // the plan asks for no such pass
+  }
+}
+
+template <int GR, bool ZP>
+static int int4_mma_launch_rows(const Int4MmaParams& p, const Int4MmaPlan& pl, int dev, int num_sms, uint8_t* staged, int* exponents, cudaStream_t stream) {
+  switch (pl.n) {
+    case 16: return int4_mma_launch<16, GR, ZP>(p, pl, dev, num_sms, staged, exponents, stream);
+    case 32: return int4_mma_launch<32, GR, ZP>(p, pl, dev, num_sms, staged, exponents, stream);
+    case 48: return int4_mma_launch<48, GR, ZP>(p, pl, dev, num_sms, staged, exponents, stream);
+    default: return int4_mma_launch<64, GR, ZP>(p, pl, dev, num_sms, staged, exponents, stream);
+  }
+}
+
+template <bool ZP>
+static int int4_mma_launch_group(const Int4MmaParams& p, const Int4MmaPlan& pl, int group, int dev, int num_sms, uint8_t* staged, int* exponents, cudaStream_t stream) {
+  switch (group) {
+    case 32: return int4_mma_launch_rows<32, ZP>(p, pl, dev, num_sms, staged, exponents, stream);
+    case 64: return int4_mma_launch_rows<64, ZP>(p, pl, dev, num_sms, staged, exponents, stream);
+    default: return int4_mma_launch_rows<128, ZP>(p, pl, dev, num_sms, staged, exponents, stream);
+  }
+}
+
 // ---- beam step ----------------------------------------------------------------------------------
 static int beam_element_bytes(int dtype) { return dtype == FMMS_F32 ? 4 : 2; }
 
@@ -140,24 +227,6 @@ static size_t beam_workspace(int R, int K, int V, int N, int dtype) {
   return parts * N * 8 + parts * 8 + parts * 4;
 }
 
-template <typename... KArgs, typename... Args>
-static int launch_behind(void (*kernel)(KArgs...), dim3 grid, int threads, cudaStream_t stream, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
-    cudaGetLastError();
-    return kErrCuda;
-  }
-  return kOk;
-}
-
 }  // namespace fmms
 
 using namespace fmms;
@@ -167,6 +236,10 @@ extern "C" {
 int fmms_query_int4_workspace(int V, int D, int group, int B, size_t* bytes) {
   if (!bytes || V <= 0 || D <= 0 || B <= 0) return FMMS_ERR_BAD_ARG;
   if (!int4_group_ok(group, D)) return FMMS_ERR_UNSUPPORTED;
+  if (B > kInt4VectorRows) {
+    *bytes = int4_mma_workspace(D, B, group);
+    return FMMS_OK;
+  }
   Int4Plan pl;
   const int rc = int4_plan(pl, D, B, group);
   if (rc == kOk) *bytes = int4_workspace(pl, V, B);
@@ -175,7 +248,7 @@ int fmms_query_int4_workspace(int V, int D, int group, int B, size_t* bytes) {
 
 int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void* qweight, const void* scales, int scale_dtype,
                      const void* zeros, int V, int D, int group, int B, void* out, int out_dtype, long long out_stride,
-                     void* workspace, size_t workspace_bytes, void* stream) {
+                     void* workspace, size_t workspace_bytes, int* status_dev, void* stream) {
   if (!x || !qweight || !scales || !out || V <= 0 || D <= 0 || B <= 0) return FMMS_ERR_BAD_ARG;
   if ((x_dtype != FMMS_BF16 && x_dtype != FMMS_F16) || (scale_dtype != FMMS_BF16 && scale_dtype != FMMS_F16) ||
       out_dtype < FMMS_BF16 || out_dtype > FMMS_F32)
@@ -184,10 +257,16 @@ int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void*
   if (!int4_group_ok(group, D)) return FMMS_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(qweight) | reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(zeros)) & 15)
     return FMMS_ERR_UNSUPPORTED;
-  Int4Plan pl;
-  int rc = int4_plan(pl, D, B, group);
+  const bool mma = B > kInt4VectorRows;
+  Int4Plan pl = {};
+  Int4MmaPlan mp = {};
+  int rc = kOk;
+  if (mma)
+    int4_mma_plan(mp, D, B, group, zeros != nullptr);
+  else
+    rc = int4_plan(pl, D, B, group);
   if (rc != kOk) return rc;
-  const size_t need = int4_workspace(pl, V, B);
+  const size_t need = mma ? int4_mma_workspace(D, B, group) : int4_workspace(pl, V, B);
   if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need)) return FMMS_ERR_WORKSPACE;
   int dev = 0, num_sms = 0;
   rc = decode_num_sms(&dev, &num_sms);
@@ -210,18 +289,35 @@ int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void*
   p.s_bf16 = scale_dtype == FMMS_BF16;
   p.out_kind = out_dtype - FMMS_BF16;
   p.x_pairs = (reinterpret_cast<uintptr_t>(x) & 3) == 0 && x_stride % 2 == 0;
+  p.group_units = group > kInt4Unit ? group / kInt4Unit : 1;
+  p.all_units = (D + kInt4Unit - 1) / kInt4Unit;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (mma) {
+    Int4MmaParams m = {};
+    m.base = p;
+    uint8_t* staged = reinterpret_cast<uint8_t*>(workspace);
+    int* exponents = reinterpret_cast<int*>(staged + (size_t)mp.passes * mp.row_steps * int4_x_bytes(mp.n, group < kInt4Unit ? group : kInt4Unit));
+    m.staged = staged;
+    m.exponents = exponents;
+    m.n = mp.n;
+    m.row_steps = mp.row_steps;
+    m.x_stages = mp.x_stages;
+    m.ring_off = mp.ring_off;
+    m.scale_off = mp.scale_off;
+    m.idesc = (1u << 4) | ((uint32_t)(mp.n >> 3) << 17) | ((128u >> 4) << 24);  // fp32 sums of fp16 products, 128 x n
+    m.status_dev = status_dev;
+    return zeros ? int4_mma_launch_group<true>(m, mp, group, dev, num_sms, staged, exponents, s)
+                 : int4_mma_launch_group<false>(m, mp, group, dev, num_sms, staged, exponents, s);
+  }
   for (p.log_rows = 0; (1 << p.log_rows) < min(B, pl.nt * 8); ++p.log_rows) {
   }
-  p.xs32_off = pl.xs32_off;
   p.partial = reinterpret_cast<float*>(workspace);
-  p.group_units = group > kInt4Unit ? group / kInt4Unit : 1;
   p.phases = pl.phases;
   p.units = pl.units;
-  p.all_units = pl.all_units;
   p.xs_off = pl.xs_off;
+  p.xs32_off = pl.xs32_off;
   p.ring_off = pl.ring_off;
   p.piece_off = pl.piece_off;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return zeros ? int4_launch_group<true>(p, pl, group, dev, num_sms, s) : int4_launch_group<false>(p, pl, group, dev, num_sms, s);
 }
 
@@ -273,7 +369,7 @@ int fmms_beam_step(const void* logits, int dtype, long long stride_r, long long 
   else
     beam_part_kernel<float><<<grid, kBeamThreads, 0, s>>>(p);
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
-  return launch_behind(beam_merge_kernel, dim3((unsigned)R), kBeamThreads, s, p);
+  return launch_behind(beam_merge_kernel, dim3((unsigned)R), kBeamThreads, 0, s, p);
 }
 
 int fmms_reorder_beams(const fmms_beam_state_t* states, int n_states, const void* parents, int parents_bytes, int R, int K,

@@ -178,6 +178,8 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
 
 
 def _launch(x, stride, weight, b, out, out_stride, index):
+    from .core import _status_word  # core is imported first
+
     qw, scales, scale_dtype, zeros, rows, cols, group = weight._args
     key = (rows, cols, group, b)
     nbytes = _ws_bytes.get(key)
@@ -188,4 +190,4 @@ def _launch(x, stride, weight, b, out, out_stride, index):
     return _lib.load().fmms_int4_linear(
         x.data_ptr(), _DTYPES[x.dtype], stride, qw, scales, scale_dtype, zeros, rows, cols, group, b,
         out.data_ptr(), _DTYPES[out.dtype], out_stride, ws.data_ptr() if nbytes else None, nbytes,
-        torch._C._cuda_getCurrentRawStream(index))
+        _status_word(x.device).data_ptr(), torch._C._cuda_getCurrentRawStream(index))

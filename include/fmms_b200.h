@@ -388,7 +388,8 @@ int fmms_static_reset(void* stream);
  */
 int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void* qweight, const void* scales,
                      int scale_dtype, const void* zeros, int V, int D, int group, int B, void* out, int out_dtype,
-                     long long out_stride, void* workspace, size_t workspace_bytes, void* stream);
+                     long long out_stride, void* workspace, size_t workspace_bytes, int* status_dev,
+                     void* stream);
 int fmms_query_int4_workspace(int V, int D, int group, int B, size_t* bytes);
 
 /*

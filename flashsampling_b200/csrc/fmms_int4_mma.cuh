@@ -128,11 +128,36 @@ __global__ void __launch_bounds__(256) int4_stage_x_kernel(const Int4MmaParams p
   }
 }
 
-__device__ __forceinline__ void tmem_store_operand(uint32_t taddr, const uint32_t (&r)[16]) {
+// Four words of codes (64 columns of 16 rows, over the warp) as fp16 subnormals: per word the operands of a 16 x 16 product.
+// Masked inside the statement, so that the results are made where the store wants them.
+__device__ __forceinline__ void tmem_store_codes(uint32_t taddr, uint4 w) {
   asm volatile(
-      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      "{\n\t"
+      ".reg .b32 s0, s1, s2, s3;\n\t"
+      ".reg .b32 a<16>;\n\t"
+      "shr.u32 s0, %1, 8;\n\t"
+      "shr.u32 s1, %2, 8;\n\t"
+      "shr.u32 s2, %3, 8;\n\t"
+      "shr.u32 s3, %4, 8;\n\t"
+      "and.b32 a0, %1, 0x000f000f;\n\t"
+      "and.b32 a1, %1, 0x00f000f0;\n\t"
+      "and.b32 a2, s0, 0x000f000f;\n\t"
+      "and.b32 a3, s0, 0x00f000f0;\n\t"
+      "and.b32 a4, %2, 0x000f000f;\n\t"
+      "and.b32 a5, %2, 0x00f000f0;\n\t"
+      "and.b32 a6, s1, 0x000f000f;\n\t"
+      "and.b32 a7, s1, 0x00f000f0;\n\t"
+      "and.b32 a8, %3, 0x000f000f;\n\t"
+      "and.b32 a9, %3, 0x00f000f0;\n\t"
+      "and.b32 a10, s2, 0x000f000f;\n\t"
+      "and.b32 a11, s2, 0x00f000f0;\n\t"
+      "and.b32 a12, %4, 0x000f000f;\n\t"
+      "and.b32 a13, %4, 0x00f000f0;\n\t"
+      "and.b32 a14, s3, 0x000f000f;\n\t"
+      "and.b32 a15, s3, 0x00f000f0;\n\t"
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {a0, a1, a2, a3, a4, a5, a6, a7, a8, a9, a10, a11, a12, a13, a14, a15};\n\t"
+      "}" ::"r"(taddr),
+      "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
       : "memory");
 }
 
@@ -305,20 +330,8 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
 #pragma unroll
       for (int i = 0; i < kStepU; ++i)
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const uint4 w4 = *reinterpret_cast<const uint4*>(src + i * 1024 + m * 512 + lane * 16);
-          const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-          uint32_t r[16];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t w8 = w[j] >> 8;
-            r[4 * j] = w[j] & 0x000f000fu;
-            r[4 * j + 1] = w[j] & 0x00f000f0u;
-            r[4 * j + 2] = w8 & 0x000f000fu;
-            r[4 * j + 3] = w8 & 0x00f000f0u;
-          }
-          if (mine > m * 4) tmem_store_operand(at + ((uint32_t)(m * 16) << 16) + i * 64, r);
-        }
+        for (int m = 0; m < 2; ++m)
+          if (mine > m * 4) tmem_store_codes(at + ((uint32_t)(m * 16) << 16) + i * 64, *reinterpret_cast<const uint4*>(src + i * 1024 + m * 512 + lane * 16));
       if constexpr (ZP) {
 #pragma unroll
         for (int j = 0; j < kZeroGroups; ++j)
@@ -330,11 +343,11 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
           }
         __syncwarp();  // everybody has read the slot's zeros
       }
-      fetch();
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&a_full[a]);
+      fetch();
       if (++slot == kInt4MmaRing) slot = 0;
     }
   } else if (warp < kInt4MmaWeightWarps + kInt4MmaSumWarps) {
@@ -376,6 +389,10 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
     const int place = (r16 & 7) * 2 + (r16 >> 3);    // within the 16 scales of a group
     const float row_factor = r16 >= 8 ? 0.0625f : 1.f;  // the upper rows are multiplied as 16 times their codes
     const int nb = min(NC, q.B - pass * p.n);
+    // what brings column first_col + lane back to its row of x
+    float down = 0.f;
+    if (lane < kCols && first_col + lane < nb)
+      down = __uint_as_float((uint32_t)(127 - p.exponents[pass * kInt4MmaPass + first_col + lane]) << 23);
     int slot = 0, d = 0, dround = 0;
 #pragma unroll 1
     for (int block = 0; block < blocks; ++block) {
@@ -419,14 +436,10 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
         }
       }
       const int v = (t_begin + block * 8 + quad + tile_of * 4) * kInt4Tile + r16;
-      if (there && v < q.V) {
 #pragma unroll
-        for (int i = 0; i < kCols; ++i)
-          if (const int n = first_col + i; n < nb) {
-            const int e = p.exponents[pass * kInt4MmaPass + n];
-            const float y = (i & 1) ? tot[i / 2].y : tot[i / 2].x;
-            int4_store(q, pass * p.n + n, v, y * 0x1p24f * __uint_as_float((uint32_t)(127 - e) << 23));
-          }
+      for (int i = 0; i < kCols; ++i) {
+        const float y = ((i & 1) ? tot[i / 2].y : tot[i / 2].x) * 0x1p24f * __shfl_sync(0xffffffffu, down, i);
+        if (there && v < q.V && first_col + i < nb) int4_store(q, pass * p.n + first_col + i, v, y);
       }
     }
   } else if (warp == kInt4MmaWeightWarps + kInt4MmaSumWarps) {

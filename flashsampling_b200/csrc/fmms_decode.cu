@@ -15,7 +15,6 @@
 namespace fmms {
 
 constexpr int kDecodeMaxDevices = 16;
-constexpr int kInt4VectorRows = 8;  // rows of x up to which the products go to mma.sync
 constexpr int kInt4SmemLimit = 230000;  // of 232448 bytes a CTA may have; the rest: static shared memory
 
 static int decode_num_sms(int* dev_out, int* sms_out) {
@@ -58,55 +57,45 @@ static int launch_behind(void (*kernel)(KArgs...), dim3 grid, int threads, int s
 
 // ---- products with 4-bit weights ----------------------------------------------------------------
 struct Int4Plan {
-  int nt, warps, phases, units, all_units, smem;
+  int phases, units, all_units, smem;
   int xs_off, xs32_off, ring_off, piece_off;
 };
 
 static int int4_smem(Int4Plan& pl, int group) {
-  int off = pl.units * 2 * pl.nt * 1024;
+  int off = pl.units * 2 * 1024;
   pl.xs_off = off;
-  off += (pl.units * int4_unit_groups(group) * pl.nt * 32 + 127) / 128 * 128;
+  off += (pl.units * int4_unit_groups(group) * kInt4Rows * 4 + 127) / 128 * 128;
   pl.xs32_off = off;
-  if (group > 32) off += pl.units * 4 * pl.nt * 32;
+  if (group > 32) off += pl.units * 4 * kInt4Rows * 4;
   pl.piece_off = off;
-  off += pl.warps * 2 * pl.nt * 512;
+  off += kInt4Warps * 2 * 512;
   pl.ring_off = off;
-  off += pl.warps * kInt4Stages * int4_stage_bytes(group);
+  off += kInt4Warps * kInt4Stages * int4_stage_bytes(group);
   pl.smem = off;
   return off;
 }
 
-// Blocks of eight rows of x per pass, warps, and the phases x takes.  16 warps hide the products' latency best (head of
-// 151936 x 4096, B = 1: 55.9 us against 57.7 with 8), but their larger buffers leave less room for x: up to 16 rows run
-// with 8 warps where those, and not 16, take all of x at once (the same head, B = 16: 93 us against 110; 262208 x 5376,
-// which takes several phases either way: 250 against 201).  More rows need the registers of 8 warps.
-static int int4_plan(Int4Plan& pl, int D, int B, int group) {
+// As few phases as shared memory allows: rows of up to some 7000 columns take one.
+static int int4_plan(Int4Plan& pl, int D, int group) {
   pl.all_units = (D + kInt4Unit - 1) / kInt4Unit;
-  pl.nt = B <= 8 ? 1 : B <= 16 ? 2 : 4;
-  auto fits = [&](int warps, int phases) {
-    pl.warps = warps;
-    pl.phases = phases;
-    pl.units = (pl.all_units + phases - 1) / phases;
-    return (phases - 1) * pl.units < pl.all_units &&  // the last phase is not empty
-           int4_smem(pl, group) <= kInt4SmemLimit;
-  };
-  if (pl.nt == 2 && !fits(16, 1) && fits(8, 1)) return kOk;
-  for (int phases = 1; phases <= pl.all_units; ++phases)
-    if (fits(pl.nt == 4 ? 8 : 16, phases)) return kOk;
+  for (pl.phases = 1; pl.phases <= pl.all_units; ++pl.phases) {
+    pl.units = (pl.all_units + pl.phases - 1) / pl.phases;
+    if ((pl.phases - 1) * pl.units < pl.all_units &&  // the last phase is not empty
+        int4_smem(pl, group) <= kInt4SmemLimit)
+      return kOk;
+  }
   return kErrUnsupported;
 }
 
 static bool int4_group_ok(int group, int D) { return (group == 32 || group == 64 || (group > 0 && group % kInt4Unit == 0)) && D % group == 0; }
 
-static size_t int4_workspace(const Int4Plan& pl, int V, int B) {
-  if (pl.phases == 1) return 0;
-  const size_t tiles = (V + kInt4Tile - 1) / kInt4Tile, blocks = (B + pl.nt * 8 - 1) / (pl.nt * 8);
-  return blocks * (tiles + 1) * pl.nt * 512;
+static size_t int4_workspace(const Int4Plan& pl, int V) {
+  return pl.phases == 1 ? 0 : (size_t)((V + kInt4Tile - 1) / kInt4Tile) * 512;
 }
 
-template <int NT, int GR, bool ZP, int W>
+template <int GR, bool ZP>
 static int int4_launch(const Int4Params& p, const Int4Plan& pl, int dev, int num_sms, cudaStream_t stream) {
-  auto* kernel = int4_linear_kernel<NT, GR, ZP, W>;
+  auto* kernel = int4_linear_kernel<GR, ZP>;
   static std::atomic<bool> ready[kDecodeMaxDevices];
   if (!ready[dev].load(std::memory_order_acquire)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kInt4SmemLimit) != cudaSuccess) {
@@ -115,30 +104,20 @@ static int int4_launch(const Int4Params& p, const Int4Plan& pl, int dev, int num
     }
     ready[dev].store(true, std::memory_order_release);
   }
-  const dim3 grid((unsigned)min(p.tiles, num_sms), (unsigned)((p.B + NT * 8 - 1) / (NT * 8)));
-  kernel<<<grid, W * 32, pl.smem, stream>>>(p);
+  kernel<<<min(p.tiles, num_sms), kInt4Warps * 32, pl.smem, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
-}
-
-template <int GR, bool ZP>
-static int int4_launch_rows(const Int4Params& p, const Int4Plan& pl, int dev, int num_sms, cudaStream_t stream) {
-  switch (pl.nt) {
-    case 1: return int4_launch<1, GR, ZP, 16>(p, pl, dev, num_sms, stream);
-    case 2: return pl.warps == 8 ? int4_launch<2, GR, ZP, 8>(p, pl, dev, num_sms, stream) : int4_launch<2, GR, ZP, 16>(p, pl, dev, num_sms, stream);
-    default: return int4_launch<4, GR, ZP, 8>(p, pl, dev, num_sms, stream);
-  }
 }
 
 template <bool ZP>
 static int int4_launch_group(const Int4Params& p, const Int4Plan& pl, int group, int dev, int num_sms, cudaStream_t stream) {
   switch (group) {
-    case 32: return int4_launch_rows<32, ZP>(p, pl, dev, num_sms, stream);
-    case 64: return int4_launch_rows<64, ZP>(p, pl, dev, num_sms, stream);
-    default: return int4_launch_rows<128, ZP>(p, pl, dev, num_sms, stream);
+    case 32: return int4_launch<32, ZP>(p, pl, dev, num_sms, stream);
+    case 64: return int4_launch<64, ZP>(p, pl, dev, num_sms, stream);
+    default: return int4_launch<128, ZP>(p, pl, dev, num_sms, stream);
   }
 }
 
-// The tensor-core variant: rows of x in a pass, and the stages of x that fit beside the rings.
+// ---- more than eight rows: fmms_int4_mma.cuh.  Rows of x in a pass, and the stages of x that fit beside the rings.
 struct Int4MmaPlan {
   int n, passes, row_steps, x_stages, ring_off, scale_off, smem;
 };
@@ -236,13 +215,13 @@ extern "C" {
 int fmms_query_int4_workspace(int V, int D, int group, int B, size_t* bytes) {
   if (!bytes || V <= 0 || D <= 0 || B <= 0) return FMMS_ERR_BAD_ARG;
   if (!int4_group_ok(group, D)) return FMMS_ERR_UNSUPPORTED;
-  if (B > kInt4VectorRows) {
+  if (B > kInt4Rows) {
     *bytes = int4_mma_workspace(D, B, group);
     return FMMS_OK;
   }
   Int4Plan pl;
-  const int rc = int4_plan(pl, D, B, group);
-  if (rc == kOk) *bytes = int4_workspace(pl, V, B);
+  const int rc = int4_plan(pl, D, group);
+  if (rc == kOk) *bytes = int4_workspace(pl, V);
   return rc;
 }
 
@@ -257,16 +236,16 @@ int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void*
   if (!int4_group_ok(group, D)) return FMMS_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(qweight) | reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(zeros)) & 15)
     return FMMS_ERR_UNSUPPORTED;
-  const bool mma = B > kInt4VectorRows;
+  const bool mma = B > kInt4Rows;
   Int4Plan pl = {};
   Int4MmaPlan mp = {};
   int rc = kOk;
   if (mma)
     int4_mma_plan(mp, D, B, group, zeros != nullptr);
   else
-    rc = int4_plan(pl, D, B, group);
+    rc = int4_plan(pl, D, group);
   if (rc != kOk) return rc;
-  const size_t need = mma ? int4_mma_workspace(D, B, group) : int4_workspace(pl, V, B);
+  const size_t need = mma ? int4_mma_workspace(D, B, group) : int4_workspace(pl, V);
   if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need)) return FMMS_ERR_WORKSPACE;
   int dev = 0, num_sms = 0;
   rc = decode_num_sms(&dev, &num_sms);
@@ -309,7 +288,7 @@ int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void*
     return zeros ? int4_mma_launch_group<true>(m, mp, group, dev, num_sms, staged, exponents, s)
                  : int4_mma_launch_group<false>(m, mp, group, dev, num_sms, staged, exponents, s);
   }
-  for (p.log_rows = 0; (1 << p.log_rows) < min(B, pl.nt * 8); ++p.log_rows) {
+  for (p.log_rows = 0; (1 << p.log_rows) < B; ++p.log_rows) {
   }
   p.partial = reinterpret_cast<float*>(workspace);
   p.phases = pl.phases;

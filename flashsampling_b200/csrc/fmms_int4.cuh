@@ -1,4 +1,4 @@
-// Products with 4-bit weights: out[b, v] = sum_k x[b, k] (q[v, k] - z[v, g(k)]) s[v, g(k)], g(k) = k / group.
+// Products with 4-bit weights for up to eight rows of x: out[b, v] = sum_k x[b, k] (q[v, k] - z[v, g(k)]) s[v, g(k)], g(k) = k / group.
 //
 // For a few rows of x the work is the stream of the weight: half a byte and 2 B flops per element.  The arithmetic per
 // streamed byte is therefore kept small instead of the arithmetic per product:
@@ -35,6 +35,8 @@ namespace fmms {
 
 constexpr int kInt4Tile = 16;    // weight rows of a tile
 constexpr int kInt4Chunk = 64;   // columns of a chunk: 512 bytes of a tile
+constexpr int kInt4Rows = 8;     // rows of x, at most (more: fmms_int4_mma.cuh)
+constexpr int kInt4Warps = 16;
 constexpr int kInt4Stages = 3;   // units in a warp's ring (4 measured the same with 8 warps and worse with 16)
 constexpr int kInt4Unit = 128;   // columns a warp fetches at a time; larger groups apply their scale to several units
 __host__ __device__ constexpr int int4_unit_groups(int group) { return group < kInt4Unit ? kInt4Unit / group : 1; }
@@ -48,7 +50,7 @@ struct Int4Params {
   const uint8_t* zeros;        // [tiles][groups][8][2], or null: 8
   void* out;
   long long out_stride;        // elements between rows of out
-  float* partial;              // [row blocks][tiles][NT * 128], several phases only
+  float* partial;              // [tiles][128], several phases only
   int V, D, B;
   int tiles, chunks, groups;
   int x_bf16, s_bf16, out_kind;  // out_kind: 0 bf16, 1 fp16, 2 fp32
@@ -111,9 +113,9 @@ __device__ __forceinline__ void int4_store(const Int4Params& p, int b, int v, fl
     reinterpret_cast<float*>(p.out)[at] = y;
 }
 
-// NT: blocks of eight rows of x; GR: columns of a group, at most 128; ZP: zero points given; W: warps.
-template <int NT, int GR, bool ZP, int W>
-__global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params p) {
+// GR: columns of a group, at most 128; ZP: zero points given.
+template <int GR, bool ZP>
+__global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_linear_kernel(const Int4Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kChunks = kInt4Unit / kInt4Chunk, kGroups = int4_unit_groups(GR);  // of a unit
   constexpr int kStage = int4_stage_bytes(GR), S = kInt4Stages;
@@ -121,22 +123,22 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
   constexpr int kScaleCopy = kGroups == 4 ? 8 : 4;                    // bytes a lane copies of the scales
   constexpr int kScaleLanes = kGroups * 32 / kScaleCopy;              // lanes of one tile
   constexpr int kZeroLanes = kGroups * 4;
-  __shared__ unsigned int warp_max[W * NT * 8];
-  __shared__ int row_exp[NT * 8];  // x went in times two to this
+  __shared__ unsigned int warp_max[kInt4Warps * kInt4Rows];
+  __shared__ int row_exp[kInt4Rows];  // x went in times two to this
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int b0 = blockIdx.y * NT * 8, nb = min(NT * 8, p.B - b0);
+  const int nb = p.B;
 
   uint4* xfrag = reinterpret_cast<uint4*>(smem);
-  float* xs = reinterpret_cast<float*>(smem + p.xs_off);      // [groups of a phase][NT * 8]
+  float* xs = reinterpret_cast<float*>(smem + p.xs_off);      // [groups of a phase][kInt4Rows]
   float* xs32 = reinterpret_cast<float*>(smem + p.xs32_off);  // the same for 32 columns each (groups of 32: xs)
-  float* pieces = reinterpret_cast<float*>(smem + p.piece_off);  // [warps][2 * NT * 4][32]
+  float* pieces = reinterpret_cast<float*>(smem + p.piece_off);  // [warps][8][32]
   const uint8_t* ring = smem + p.ring_off + warp * (S * kStage);
   const uint32_t ring_at = smem_u32(ring);
 
   // x: a thread has one row and one t, and 8 of every 32 columns: the 16 bytes of one lane's operands.  The first loads go
   // out before anything else, the ring's behind them.
-  const int stride = (W * 8) >> p.log_rows, first_block = (tid >> 2) >> p.log_rows;
+  const int stride = (kInt4Warps * 8) >> p.log_rows, first_block = (tid >> 2) >> p.log_rows;
   const int row = (tid >> 2) & ((1 << p.log_rows) - 1);
   constexpr int kAhead = 4;  // loads in flight
   uint4 raw[kAhead];
@@ -145,7 +147,7 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
     for (int i = 0; i < kAhead; ++i) {
       const int blk = from + i * stride;
       raw[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (row < nb && blk < blocks && k_begin + blk * 32 < p.D) raw[i] = int4_load_x(p, b0 + row, k_begin + blk * 32 + t * 2);
+      if (row < nb && blk < blocks && k_begin + blk * 32 < p.D) raw[i] = int4_load_x(p, row, k_begin + blk * 32 + t * 2);
     }
   };
   load_blocks(0, p.units * (kInt4Unit / 32), first_block);
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
   // this CTA's tiles in pairs, and the warps' parts of them; position = pair * units + unit
   const int t_each = p.tiles / (int)gridDim.x, t_rest = p.tiles - t_each * (int)gridDim.x;
   const int t_begin = t_each * (int)blockIdx.x + min((int)blockIdx.x, t_rest), t_end = t_begin + t_each + ((int)blockIdx.x < t_rest);
-  const int span = (t_end - t_begin + 1) / 2 * p.units, s_each = span / W, s_rest = span - s_each * W;
+  const int span = (t_end - t_begin + 1) / 2 * p.units, s_each = span / kInt4Warps, s_rest = span - s_each * kInt4Warps;
   auto part = [&](int w) { return s_each * w + min(w, s_rest); };
   const int begin = part(warp), end = part(warp + 1);
   const int p_first = begin / p.units, p_last = (end - 1) / p.units;
@@ -224,14 +226,12 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
   for (int i = 0; i < S - 1; ++i) fetch();
 
   auto pow2 = [](int e) { return __uint_as_float((uint32_t)(e + 127) << 23); };
-  float tot[2][NT][4];
+  float tot[2][4];
   auto clear = [&] {
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) tot[m][nt][j] = 0.f;
+      for (int j = 0; j < 4; ++j) tot[m][j] = 0.f;
   };
   auto write_out = [&](int pr) {
     const int tile = t_begin + pr * 2;
@@ -239,12 +239,10 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
     for (int m = 0; m < 2; ++m)
       if (tile + m < t_end)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int n = nt * 8 + t * 2 + (j & 1), v = (tile + m) * kInt4Tile + g + ((j & 2) ? 8 : 0);
-            if (n < nb && v < p.V) int4_store(p, b0 + n, v, tot[m][nt][j]);
-          }
+        for (int j = 0; j < 4; ++j) {
+          const int n = t * 2 + (j & 1), v = (tile + m) * kInt4Tile + g + ((j & 2) ? 8 : 0);
+          if (n < nb && v < p.V) int4_store(p, n, v, tot[m][j]);
+        }
   };
   int slot = 0;
 
@@ -252,7 +250,7 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
     // x as it is into the places of its operands, with the maximum of each row on the way; then, each thread what it
     // wrote itself, in fp16, and the sums over the groups
     const int k_begin = phase * p.units * kInt4Unit, blocks = min(p.units, p.all_units - phase * p.units) * (kInt4Unit / 32);
-    uint4* const mine = xfrag + (row >> 3) * 32 + (row & 7) * 4 + t;
+    uint4* const mine = xfrag + row * 4 + t;
     if (phase > 0) {
       load_blocks(k_begin, blocks, first_block);
       __syncthreads();  // the phase before has been read
@@ -264,7 +262,7 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int blk = from + i * stride;
-        if (row < nb && blk < blocks) mine[blk * (NT * 32)] = raw[i];
+        if (row < nb && blk < blocks) mine[blk * 32] = raw[i];
         m = __vmaxu2(m, __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu), __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu)));
       }
     }
@@ -275,13 +273,11 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1)  // lanes of the same row
         if (off < 4 || off >= (4 << p.log_rows)) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
-      if (lane < (4 << p.log_rows) && t == 0) warp_max[warp * (NT * 8) + row] = m;
+      if (lane < (4 << p.log_rows) && t == 0) warp_max[warp * kInt4Rows + row] = m;
       __syncthreads();
       m = 0u;
-      // a warp has eight rows or all of them: this thread's row is in every `every`-th warp
-      const int every = p.log_rows > 3 ? 1 << (p.log_rows - 3) : 1;
 #pragma unroll 4
-      for (int w = (row >> 3) & (every - 1); w < W; w += every) m = max(m, warp_max[w * (NT * 8) + row]);
+      for (int w = 0; w < kInt4Warps; ++w) m = max(m, warp_max[w * kInt4Rows + row]);
       if (m != 0u) exponent = min(14 - ((int)(m >> 7) - 127), 120);
     }
     if (first_block == 0 && t == 0 && row < nb) row_exp[row] = exponent;
@@ -294,7 +290,7 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
 #pragma unroll
       for (int i = 0; i < kConvert; ++i) {
         x4[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (row < nb && from + i * stride < blocks) x4[i] = mine[(from + i * stride) * (NT * 32)];
+        if (row < nb && from + i * stride < blocks) x4[i] = mine[(from + i * stride) * 32];
       }
 #pragma unroll
       for (int i = 0; i < kConvert; ++i) {
@@ -317,38 +313,33 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
       for (int i = 0; i < kConvert; ++i) {
         const int blk = from + i * stride;
         if (row >= nb || blk >= blocks) continue;
-        if (p.x_bf16) mine[blk * (NT * 32)] = x4[i];
+        if (p.x_bf16) mine[blk * 32] = x4[i];
         // in units of the operands; without zero points times 8
-        if (t == 0) (GR == 32 ? xs : xs32)[blk * (NT * 8) + row] = s[i] * (ZP ? -0x1p-24f : -0x1p-21f);
+        if (t == 0) (GR == 32 ? xs : xs32)[blk * kInt4Rows + row] = s[i] * (ZP ? -0x1p-24f : -0x1p-21f);
       }
     }
     __syncthreads();
     if constexpr (GR > 32) {
-      for (int i = tid; i < blocks / (GR / 32) * (NT * 8); i += W * 32) {
+      for (int i = tid; i < blocks / (GR / 32) * kInt4Rows; i += kInt4Warps * 32) {
         float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < GR / 32; ++j) s += xs32[(i / (NT * 8) * (GR / 32) + j) * (NT * 8) + i % (NT * 8)];
+        for (int j = 0; j < GR / 32; ++j) s += xs32[(i / kInt4Rows * (GR / 32) + j) * kInt4Rows + i % kInt4Rows];
         xs[i] = s;
       }
       __syncthreads();
     }
 
-    float down[NT][2];  // from the units of the sums to the result
+    float down[2];  // from the units of the sums to the result
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int n = nt * 8 + t * 2 + i;
-        down[nt][i] = n < nb ? pow2(-row_exp[n]) : 0.f;
-      }
+    for (int i = 0; i < 2; ++i) down[i] = t * 2 + i < nb ? pow2(-row_exp[t * 2 + i]) : 0.f;
 
     clear();
     for (int pr = p_first; pr <= p_last && begin < end; ++pr) {
       int u, hi;
       unit_range(phase, pr, u, hi);
       if (u >= hi) continue;
-      const uint4* xp = xfrag + u * (kChunks * 2 * NT * 32) + lane;
-      const float* xsp = xs + u * (kGroups * NT * 8) + t * 2;
+      const uint4* xp = xfrag + u * (kChunks * 2 * 32) + lane;
+      const float* xsp = xs + u * (kGroups * kInt4Rows) + t * 2;
       for (; u < hi; ++u) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
         __syncwarp();  // scales and zeros were copied by other lanes; and everybody is done with the slot before this one
@@ -357,7 +348,7 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
         const uint4* qsrc = reinterpret_cast<const uint4*>(src) + lane;
         const uint32_t* ssrc = reinterpret_cast<const uint32_t*>(src + kScaleOff) + g;
         const uint16_t* zsrc = reinterpret_cast<const uint16_t*>(src + kZeroOff) + g;
-        float acc[2][NT][4];
+        float acc[2][4];
 #pragma unroll
         for (int cc = 0; cc < kChunks; ++cc) {
           uint32_t qw[2][4];
@@ -374,25 +365,20 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
             constexpr int kPairs = GR / 32;  // of a group
             const int gi = (cc * 2 + jj) / kPairs;  // group within the unit
             const bool first = (cc * 2 + jj) % kPairs == 0, last = (cc * 2 + jj) % kPairs == kPairs - 1;
-            uint4 xv[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) xv[nt] = xp[((cc * 2 + jj) * NT + nt) * 32];
+            const uint4 xv = xp[(cc * 2 + jj) * 32];
             // Two products to a chain, chains joined by rounded additions: the tensor cores cut sums off.  All first
-            // products, then all second ones: 2 NT chains in flight.
-            float c[2][NT][4];
+            // products, then all second ones.
+            float c[2][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int m = 0; m < 2; ++m) {
                 const uint32_t w = qw[m][jj * 2 + h], w8 = w >> 8;
                 const uint32_t a0 = w & 0x000f000fu, a1 = w & 0x00f000f0u, a2 = w8 & 0x000f000fu, a3 = w8 & 0x00f000f0u;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                  if (h == 0)
-                    mma_16816(c[m][nt], a0, a1, a2, a3, xv[nt].x, xv[nt].y, 0.f, 0.f, 0.f, 0.f);
-                  else
-                    mma_16816(c[m][nt], a0, a1, a2, a3, xv[nt].z, xv[nt].w, c[m][nt][0], c[m][nt][1], c[m][nt][2], c[m][nt][3]);
-                }
+                if (h == 0)
+                  mma_16816(c[m], a0, a1, a2, a3, xv.x, xv.y, 0.f, 0.f, 0.f, 0.f);
+                else
+                  mma_16816(c[m], a0, a1, a2, a3, xv.z, xv.w, c[m][0], c[m][1], c[m][2], c[m][3]);
               }
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
@@ -403,38 +389,29 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
                   z0 = (float)(z & 0xffu);
                   z1 = (float)(z >> 8) * 16.f;
                 }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                  const float2 xsum = *reinterpret_cast<const float2*>(xsp + gi * (NT * 8) + nt * 8);
-                  acc[m][nt][0] = c[m][nt][0];
-                  acc[m][nt][1] = c[m][nt][1];
-                  acc[m][nt][2] = c[m][nt][2];
-                  acc[m][nt][3] = c[m][nt][3];
-                  fma2(acc[m][nt][0], acc[m][nt][1], z0, xsum.x, xsum.y);
-                  fma2(acc[m][nt][2], acc[m][nt][3], z1, xsum.x, xsum.y);
-                }
+                const float2 xsum = *reinterpret_cast<const float2*>(xsp + gi * kInt4Rows);
+                acc[m][0] = c[m][0];
+                acc[m][1] = c[m][1];
+                acc[m][2] = c[m][2];
+                acc[m][3] = c[m][3];
+                fma2(acc[m][0], acc[m][1], z0, xsum.x, xsum.y);
+                fma2(acc[m][2], acc[m][3], z1, xsum.x, xsum.y);
               } else {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                  add2(acc[m][nt][0], acc[m][nt][1], c[m][nt][0], c[m][nt][1]);
-                  add2(acc[m][nt][2], acc[m][nt][3], c[m][nt][2], c[m][nt][3]);
-                }
+                add2(acc[m][0], acc[m][1], c[m][0], c[m][1]);
+                add2(acc[m][2], acc[m][3], c[m][2], c[m][3]);
               }
               if (last && (GR == kInt4Unit || (phase * p.units + u) * kGroups + gi < p.groups)) {
                 const uint32_t s2 = ssrc[(m * kGroups + gi) * 8];
                 const float s0 = half_bits_to_float(s2 & 0xffffu, p.s_bf16);
                 const float s1 = half_bits_to_float(s2 >> 16, p.s_bf16) * 0.0625f;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                  fma2(tot[m][nt][0], tot[m][nt][1], s0, acc[m][nt][0], acc[m][nt][1]);
-                  fma2(tot[m][nt][2], tot[m][nt][3], s1, acc[m][nt][2], acc[m][nt][3]);
-                }
+                fma2(tot[m][0], tot[m][1], s0, acc[m][0], acc[m][1]);
+                fma2(tot[m][2], tot[m][3], s1, acc[m][2], acc[m][3]);
               }
             }
           }
         }
-        xp += kChunks * 2 * NT * 32;
-        xsp += kGroups * NT * 8;
+        xp += kChunks * 2 * 32;
+        xsp += kGroups * kInt4Rows;
         if (++slot == S) slot = 0;
       }
       // the warp's part of this pair in this phase is complete
@@ -442,25 +419,23 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) tot[m][nt][j] = tot[m][nt][j] * 0x1p24f * down[nt][j & 1];
+        for (int j = 0; j < 4; ++j) tot[m][j] = tot[m][j] * 0x1p24f * down[j & 1];
       if (!has_start) {
-        float* mine = pieces + warp * (2 * NT * 128) + lane;
+        float* mine = pieces + warp * (2 * 128) + lane;
 #pragma unroll
-        for (int i = 0; i < 2 * NT * 4; ++i) {
-          const float y = tot[i / (NT * 4)][i / 4 % NT][i % 4];
+        for (int i = 0; i < 8; ++i) {
+          const float y = tot[i / 4][i % 4];
           mine[i * 32] = phase ? mine[i * 32] + y : y;
         }
         clear();
         continue;
       }
       if (p.phases > 1) {  // what the phases before left
-        float* mine = p.partial + ((size_t)blockIdx.y * (p.tiles + 1) + t_begin + pr * 2) * (NT * 128) + lane;
+        float* mine = p.partial + ((size_t)t_begin + pr * 2) * 128 + lane;
 #pragma unroll
-        for (int i = 0; i < 2 * NT * 4; ++i) {
-          if (t_begin + pr * 2 + i / (NT * 4) >= t_end) continue;
-          float& y = tot[i / (NT * 4)][i / 4 % NT][i % 4];
+        for (int i = 0; i < 8; ++i) {
+          if (t_begin + pr * 2 + i / 4 >= t_end) continue;
+          float& y = tot[i / 4][i % 4];
           if (phase) y += mine[i * 32];
           if (phase + 1 < p.phases) mine[i * 32] = y;
         }
@@ -475,11 +450,11 @@ __global__ void __launch_bounds__(W * 32, 1) int4_linear_kernel(const Int4Params
     const int pr = p_last, stop = (pr + 1) * p.units;
     if (begin <= pr * p.units && end < stop) {
 #pragma unroll 4
-      for (int w = warp + 1; w < W && part(w) < stop; ++w) {
+      for (int w = warp + 1; w < kInt4Warps && part(w) < stop; ++w) {
         if (part(w) == part(w + 1)) continue;
-        const float* other = pieces + w * (2 * NT * 128) + lane;
+        const float* other = pieces + w * (2 * 128) + lane;
 #pragma unroll
-        for (int i = 0; i < 2 * NT * 4; ++i) tot[i / (NT * 4)][i / 4 % NT][i % 4] += other[i * 32];
+        for (int i = 0; i < 8; ++i) tot[i / 4][i % 4] += other[i * 32];
       }
       write_out(pr);
     }

@@ -3,17 +3,18 @@
 // For a few rows of x the work is the stream of the weight: half a byte and 2 B flops per element.  The arithmetic per
 // streamed byte is therefore kept small instead of the arithmetic per product:
 //
-//   Integers enter the tensor cores as they are stored.  Masking a 32-bit word with 0x000f000f leaves two fp16
-//   subnormals q 2^-24, masking it with 0x00f000f0 two subnormals q 2^-20: both exact, so eight weights cost four
-//   ANDs and one shift, with no conversion and no subtraction.  The stored order puts the two nibbles of a byte into
-//   two different rows of the 16 x 16 operand, so that the factor 2^4 between the masks belongs to a whole row and
-//   joins that row's scale.
+//   Integers enter the tensor cores as they are stored.  A nibble in bits 4 to 7 of an fp16 number is the subnormal
+//   q 2^-20, exact, so eight weights cost four ANDs and three shifts, with no conversion and no subtraction.  (Bits 0 to 3,
+//   for one shift, would be exact too, but the tensor cores line products up by their exponent fields, which hide a
+//   subnormal's leading zeros: rows with their codes there came out to 1e-6, against 1e-7 in bits 4 to 7.  Subtracting the
+//   zero point first costs four fp16 operations more: 151936 x 4096 at one row took 68 us instead of 55.)  The stored order
+//   puts the two nibbles of a byte into two different rows of the 16 x 16 operand.
 //   The zero point leaves the product: sum_k x (q - z) = sum_k x q - z sum_k x.  The accumulators of a group start at
 //   -z sum_k x (the sum over the group is formed once per CTA, in fp32, from the rounded x that the products use, so the
 //   two parts cancel exactly), the scale is applied once per group in fp32, and groups add up in fp32.
-//   x becomes fp16 after a power-of-two scaling per row that puts its largest element near 2^14: bf16 and fp16 values
-//   down to 2^-28 of the row's maximum keep all their bits, smaller ones are rounded to 2^-39 of that maximum, which is
-//   below the rounding of the fp32 sums.
+//   x becomes fp16 after a power-of-two scaling per row that puts its largest element near 2^14: bf16 values down to 2^-28
+//   of the row's maximum keep all their bits, smaller ones are rounded to 2^-39 of that maximum, which is below the
+//   rounding of the fp32 sums.  fp16 goes in as it is.
 //
 // Work split.  Tiles of 16 rows are dealt to the CTAs, one per SM, in contiguous ranges; the warps of a CTA share its
 // range in equal parts that begin and end anywhere in a pair of tiles (two at a time share the operand loads of x).  A
@@ -37,7 +38,7 @@ constexpr int kInt4Tile = 16;    // weight rows of a tile
 constexpr int kInt4Chunk = 64;   // columns of a chunk: 512 bytes of a tile
 constexpr int kInt4Rows = 8;     // rows of x, at most (more: fmms_int4_mma.cuh)
 constexpr int kInt4Warps = 16;
-constexpr int kInt4Stages = 3;   // units in a warp's ring (4 measured the same with 8 warps and worse with 16)
+constexpr int kInt4Stages = 3;   // units in a warp's ring (4 measured worse)
 constexpr int kInt4Unit = 128;   // columns a warp fetches at a time; larger groups apply their scale to several units
 __host__ __device__ constexpr int int4_unit_groups(int group) { return group < kInt4Unit ? kInt4Unit / group : 1; }
 __host__ __device__ constexpr int int4_stage_bytes(int group) { return 2 * (2 * 512 + int4_unit_groups(group) * 48); }
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_linear_kernel(const I
         if (row >= nb || blk >= blocks) continue;
         if (p.x_bf16) mine[blk * 32] = x4[i];
         // in units of the operands; without zero points times 8
-        if (t == 0) (GR == 32 ? xs : xs32)[blk * kInt4Rows + row] = s[i] * (ZP ? -0x1p-24f : -0x1p-21f);
+        if (t == 0) (GR == 32 ? xs : xs32)[blk * kInt4Rows + row] = s[i] * (ZP ? -0x1p-20f : -0x1p-17f);
       }
     }
     __syncthreads();
@@ -373,8 +374,8 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_linear_kernel(const I
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int m = 0; m < 2; ++m) {
-                const uint32_t w = qw[m][jj * 2 + h], w8 = w >> 8;
-                const uint32_t a0 = w & 0x000f000fu, a1 = w & 0x00f000f0u, a2 = w8 & 0x000f000fu, a3 = w8 & 0x00f000f0u;
+                const uint32_t w = qw[m][jj * 2 + h];
+                const uint32_t a0 = (w << 4) & 0x00f000f0u, a1 = w & 0x00f000f0u, a2 = (w >> 4) & 0x00f000f0u, a3 = (w >> 8) & 0x00f000f0u;
                 if (h == 0)
                   mma_16816(c[m], a0, a1, a2, a3, xv.x, xv.y, 0.f, 0.f, 0.f, 0.f);
                 else
@@ -383,11 +384,11 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_linear_kernel(const I
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
               if (first) {
-                float z0 = 1.f, z1 = 16.f;
+                float z0 = 1.f, z1 = 1.f;
                 if constexpr (ZP) {
                   const uint32_t z = zsrc[(m * kGroups + gi) * 8];
                   z0 = (float)(z & 0xffu);
-                  z1 = (float)(z >> 8) * 16.f;
+                  z1 = (float)(z >> 8);
                 }
                 const float2 xsum = *reinterpret_cast<const float2*>(xsp + gi * kInt4Rows);
                 acc[m][0] = c[m][0];
@@ -403,7 +404,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_linear_kernel(const I
               if (last && (GR == kInt4Unit || (phase * p.units + u) * kGroups + gi < p.groups)) {
                 const uint32_t s2 = ssrc[(m * kGroups + gi) * 8];
                 const float s0 = half_bits_to_float(s2 & 0xffffu, p.s_bf16);
-                const float s1 = half_bits_to_float(s2 >> 16, p.s_bf16) * 0.0625f;
+                const float s1 = half_bits_to_float(s2 >> 16, p.s_bf16);
                 fma2(tot[m][0], tot[m][1], s0, acc[m][0], acc[m][1]);
                 fma2(tot[m][2], tot[m][3], s1, acc[m][2], acc[m][3]);
               }
@@ -419,7 +420,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_linear_kernel(const I
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) tot[m][j] = tot[m][j] * 0x1p24f * down[j & 1];
+        for (int j = 0; j < 4; ++j) tot[m][j] = tot[m][j] * 0x1p20f * down[j & 1];
       if (!has_start) {
         float* mine = pieces + warp * (2 * 128) + lane;
 #pragma unroll

@@ -2,14 +2,16 @@
 // fmms_int4.cuh, on the fifth-generation tensor cores.
 //
 // mma.sync takes eight cycles for a 16 x 16 x 8 product here, so that beyond eight rows the products and not the weight's
-// stream set its pace (151936 x 4096: 56 us for one row, 83 us for 16, 216 us for 32).  tcgen05.mma takes 128 weight
+// stream set its pace (151936 x 4096: 55 us for one row, 59 us for 8, 83 us for 16, 216 us for 32, where this kernel takes
+// 89 us and 105 us; 128256 x 8192 at 16 rows: 200 us and 145 us).  tcgen05.mma takes 128 weight
 // rows against all rows of x at once, and it reads one operand from tensor memory: the weights go from registers there,
 // in the very layout the stored order is made for (tcgen05.st .16x128b places what a lane holds of a 16 x 16 operand), and
 // never through shared memory as fp16.
 //
 // A CTA per SM has a contiguous range of tiles and takes eight of them (128 rows) at a time:
 //   warps 0-15   stream the weights through rings of asynchronous copies of their own (warp w: every second step, the
-//                tiles of tensor-memory lanes 32 (w mod 4).., half of the columns), mask the nibbles and store them
+//                tiles of tensor-memory lanes 32 (w mod 4).., half of the columns), move the nibbles to bits 4 to 7 of fp16
+//                subnormals and store them
 //   warps 16-23  read the sums of every group back, a weight row and half of the rows of x per thread: out[n] += s sum[n] in
 //                fp32
 //   warp 24      issues the products, a group of columns to an accumulator
@@ -18,7 +20,8 @@
 // and minus the sum of x over the group, cut into three fp16 parts, on the other.  That halves what the reading back
 // costs (a multiply-add per row of x and group instead of two and a load).
 // int4_stage_x writes x beforehand, as fp16 in the swizzled layout of the products with those columns behind every step.
-// Its power of two per row puts the row's largest element into [2^7, 2^8), so that a group's sum fits fp16 as well.
+// Its power of two per row puts the row's largest element into [2^7, 2^8), so that a group's sum fits fp16 as well; what lies
+// below 2^-24 of that element (2^-21 for fp16 rows) is rounded to 2^-32 of it, far below the rounding of the fp32 sums.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -133,28 +136,35 @@ __global__ void __launch_bounds__(256) int4_stage_x_kernel(const Int4MmaParams p
 __device__ __forceinline__ void tmem_store_codes(uint32_t taddr, uint4 w) {
   asm volatile(
       "{\n\t"
-      ".reg .b32 s0, s1, s2, s3;\n\t"
       ".reg .b32 a<16>;\n\t"
-      "shr.u32 s0, %1, 8;\n\t"
-      "shr.u32 s1, %2, 8;\n\t"
-      "shr.u32 s2, %3, 8;\n\t"
-      "shr.u32 s3, %4, 8;\n\t"
-      "and.b32 a0, %1, 0x000f000f;\n\t"
+      "shl.b32 a0, %1, 4;\n\t"
+      "shr.u32 a2, %1, 4;\n\t"
+      "shr.u32 a3, %1, 8;\n\t"
+      "shl.b32 a4, %2, 4;\n\t"
+      "shr.u32 a6, %2, 4;\n\t"
+      "shr.u32 a7, %2, 8;\n\t"
+      "shl.b32 a8, %3, 4;\n\t"
+      "shr.u32 a10, %3, 4;\n\t"
+      "shr.u32 a11, %3, 8;\n\t"
+      "shl.b32 a12, %4, 4;\n\t"
+      "shr.u32 a14, %4, 4;\n\t"
+      "shr.u32 a15, %4, 8;\n\t"
+      "and.b32 a0, a0, 0x00f000f0;\n\t"
       "and.b32 a1, %1, 0x00f000f0;\n\t"
-      "and.b32 a2, s0, 0x000f000f;\n\t"
-      "and.b32 a3, s0, 0x00f000f0;\n\t"
-      "and.b32 a4, %2, 0x000f000f;\n\t"
+      "and.b32 a2, a2, 0x00f000f0;\n\t"
+      "and.b32 a3, a3, 0x00f000f0;\n\t"
+      "and.b32 a4, a4, 0x00f000f0;\n\t"
       "and.b32 a5, %2, 0x00f000f0;\n\t"
-      "and.b32 a6, s1, 0x000f000f;\n\t"
-      "and.b32 a7, s1, 0x00f000f0;\n\t"
-      "and.b32 a8, %3, 0x000f000f;\n\t"
+      "and.b32 a6, a6, 0x00f000f0;\n\t"
+      "and.b32 a7, a7, 0x00f000f0;\n\t"
+      "and.b32 a8, a8, 0x00f000f0;\n\t"
       "and.b32 a9, %3, 0x00f000f0;\n\t"
-      "and.b32 a10, s2, 0x000f000f;\n\t"
-      "and.b32 a11, s2, 0x00f000f0;\n\t"
-      "and.b32 a12, %4, 0x000f000f;\n\t"
+      "and.b32 a10, a10, 0x00f000f0;\n\t"
+      "and.b32 a11, a11, 0x00f000f0;\n\t"
+      "and.b32 a12, a12, 0x00f000f0;\n\t"
       "and.b32 a13, %4, 0x00f000f0;\n\t"
-      "and.b32 a14, s3, 0x000f000f;\n\t"
-      "and.b32 a15, s3, 0x00f000f0;\n\t"
+      "and.b32 a14, a14, 0x00f000f0;\n\t"
+      "and.b32 a15, a15, 0x00f000f0;\n\t"
       "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {a0, a1, a2, a3, a4, a5, a6, a7, a8, a9, a10, a11, a12, a13, a14, a15};\n\t"
       "}" ::"r"(taddr),
       "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
@@ -304,12 +314,12 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
     };
 #pragma unroll 1
     for (int i = 0; i < kInt4MmaRing - 1; ++i) fetch();
-    // z at columns 0, 1 and 2 of a row: what lane (g, t) holds of the operand, for rows g and 8 + g (which count 16 times)
+    // z 2^-20 at columns 0, 1 and 2 of a row: what lane (g, t) holds of the operand, for rows g and 8 + g.  Above 127 that is
+    // no subnormal: the number's step doubles at 2^-13.
     const int t = lane & 3;
-    const uint32_t z_mask = t == 0 ? 0x00ff00ffu : t == 1 ? 0x000000ffu : 0u;
-    auto store_zero_points = [&](uint32_t at, uint32_t pair) {
-      tmem_store_zero_points(at, (pair & 0xffu) * 0x00010001u & z_mask, ((pair >> 8) * 0x00010001u & z_mask) << 4);
-    };
+    const uint32_t z_mask = t == 0 ? 0xffffffffu : t == 1 ? 0x0000ffffu : 0u;
+    auto zero_point = [&](uint32_t z) { return min(z << 4, (z << 3) + 1024u) * 0x00010001u & z_mask; };
+    auto store_zero_points = [&](uint32_t at, uint32_t pair) { tmem_store_zero_points(at, zero_point(pair & 0xffu), zero_point(pair >> 8)); };
     if constexpr (!ZP)
       if (warp < 4) {  // before this warp's first step, and read from step 0 on, which is its own
         store_zero_points(tmem + lanes + kZeroAt, 0x0808u);
@@ -387,7 +397,6 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
     griddep_wait();  // the exponents come from the kernel before
     const int r16 = lane & 15, tile_of = lane >> 4;  // row within its tile; first or second tile
     const int place = (r16 & 7) * 2 + (r16 >> 3);    // within the 16 scales of a group
-    const float row_factor = r16 >= 8 ? 0.0625f : 1.f;  // the upper rows are multiplied as 16 times their codes
     const int nb = min(NC, q.B - pass * p.n);
     // what brings column first_col + lane back to its row of x
     float down = 0.f;
@@ -408,7 +417,7 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
         float s[kStepG];
 #pragma unroll
         for (int gi = 0; gi < kStepG; ++gi)
-          s[gi] = row_factor * half_bits_to_float(reinterpret_cast<const uint16_t*>(ring + slot * kScaleBytes)[tile_of * (kStepG * 16) + gi * 16 + place], q.s_bf16);
+          s[gi] = half_bits_to_float(reinterpret_cast<const uint16_t*>(ring + slot * kScaleBytes)[tile_of * (kStepG * 16) + gi * 16 + place], q.s_bf16);
         if (++slot == kInt4MmaScaleRing) slot = 0;
         mbar_wait(&done[d], (uint32_t)dround & 1u, abort_flag, p.status_dev);
         tc_fence_after();
@@ -438,7 +447,7 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
       const int v = (t_begin + block * 8 + quad + tile_of * 4) * kInt4Tile + r16;
 #pragma unroll
       for (int i = 0; i < kCols; ++i) {
-        const float y = ((i & 1) ? tot[i / 2].y : tot[i / 2].x) * 0x1p24f * __shfl_sync(0xffffffffu, down, i);
+        const float y = ((i & 1) ? tot[i / 2].y : tot[i / 2].x) * 0x1p20f * __shfl_sync(0xffffffffu, down, i);
         if (there && v < q.V && first_col + i < nb) int4_store(q, pass * p.n + first_col + i, v, y);
       }
     }

@@ -125,9 +125,10 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
     """``x @ weight.T`` for bf16 or fp16 ``x [..., cols]``: ``[..., rows]`` in ``out_dtype`` (bf16, fp16 or fp32; default
     the type of ``x``), or into ``out``.
 
-    Made for the few rows of a decode step (up to 16 the call costs little more than the weight's stream; larger batches
-    run in passes of at most 32 rows).  Rows of ``x`` may be strided.  Sums are fp32 and their order is fixed.  No
-    gradients: the weight is for serving."""
+    Made for the few rows of a decode step: up to eight rows cost little more than the weight's stream, 16 to 32 rows one
+    and a half to two times that, and more than 64 (32 for groups of 32 columns) stream the weight more than once.  Rows of
+    ``x`` may be strided.  Sums are fp32 and their order is fixed: a row of ``x`` gives the same bits in every batch of up
+    to eight rows, and in every larger one.  No gradients: the weight is for serving."""
     if not isinstance(weight, Int4Weight):
         raise TypeError("weight must be an Int4Weight")
     if not (x.is_cuda and weight.qweight.is_cuda):

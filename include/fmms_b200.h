@@ -378,13 +378,15 @@ int fmms_static_reset(void* stream);
  *   zeros        the same shape in uint8, or NULL: 8 everywhere
  *   group        32, 64 or a multiple of 128 (up to D: one scale per row), a divisor of D
  *   out          [B, V] bf16, fp16 or fp32, rows `out_stride` elements apart; written once, nothing else is touched
- *   workspace    fmms_query_int4_workspace() bytes, 16-byte aligned (0 bytes, and NULL, while x fits shared memory); holds
- *                nothing between calls, need not be zeroed, and must not be used by two calls at once
+ *   workspace    fmms_query_int4_workspace() bytes, 16-byte aligned (0 bytes, and NULL, for up to eight rows that fit shared
+ *                memory); holds nothing between calls, need not be zeroed, and must not be used by two calls at once
+ *   status_dev   an int, or NULL: set to FMMS_ERR_TIMEOUT when a wait between the warps of a kernel ran out (as in the other calls)
  *
- * Sums are fp32; x is brought to fp16 with an exact power of two per row (values below 2^-28 of a row's largest
- * lose bits beyond 2^-39 of it).  A row of x that is not finite gives a row that is not finite.  The order of
- * additions is fixed: equal calls give equal bits, and a row's result does not depend on the other rows of its
- * call's batch as long as the number of rows stays within the same of the ranges 1-8, 9-16, 17 and more.
+ * Sums are fp32.  x is brought to fp16 with an exact power of two per row: values below 2^-28 of a row's largest lose bits
+ * beyond 2^-39 of it in calls of up to eight rows, values below 2^-24 (bf16; 2^-21 for fp16) bits beyond 2^-32 in larger ones.
+ * A row of x that is not finite gives a row that is not finite.  The order of additions is fixed: equal calls give equal
+ * bits, and a row's result does not depend on the other rows of its call's batch as long as the number of rows stays
+ * within 1-8, or above 8.
  */
 int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void* qweight, const void* scales,
                      int scale_dtype, const void* zeros, int V, int D, int group, int B, void* out, int out_dtype,

@@ -1,7 +1,8 @@
 """4-bit products against the dequantised weight in 64 bits.
 
-Tolerance.  Every product of a code (4 bits) with an x in fp16 is exact, and x reaches fp16 exactly unless it lies below
-2^-28 of its row's maximum (then within 2^-39 of that maximum).  What rounds are fp32 additions.  Tensor cores may
+Tolerance.  Every product of a code (4 bits) with an x in fp16 is exact.  x reaches fp16 after a power of two that puts
+its row's maximum at 2^14 or above, from nine rows on at 2^7 or above: where bits are lost, half a step of the smallest
+fp16 numbers is 2^-25, or 2^-39 and 2^-32 of that maximum.  What rounds are fp32 additions.  Tensor cores may
 truncate (2^-23 relative to the largest partial sum) and every partial sum is at most A = sum_k scale (q + zero) |x|.  An
 output passes through at most 16 additions inside a product, group / 16 products, cols / group group sums, 16 warps, 8
 CTAs, and 8 further roundings (sums of x, zero point, scales, powers of two): error <= n 2^-23 A with that n.  The
@@ -50,7 +51,7 @@ def _reference(w, x):
     xd = x.double().reshape(-1, w.cols)
     amount = xd.abs() @ (scale.abs() * (w.codes().double() + zero)).T
     n = 16 + w.group_size // 16 + w.cols // w.group_size + 16 + 8 + 8
-    tiny = xd.abs().amax(1, keepdim=True) * 2.0**-39 * (scale.abs() * 16).sum(1)
+    tiny = xd.abs().amax(1, keepdim=True) * (2.0**-39 if xd.shape[0] <= 8 else 2.0**-32) * (scale.abs() * 16).sum(1)
     shape = x.shape[:-1] + (w.rows,)
     return (xd @ wd.T).view(shape), (n * 2.0**-23 * amount + tiny).view(shape)
 
@@ -204,6 +205,87 @@ def test_same_bits_every_time_and_in_every_batch(fs):
         assert torch.equal(fs.int4_linear(x, w, out_dtype=torch.float32), first)
     for b in range(8):
         assert torch.equal(fs.int4_linear(x[b:b + 1], w, out_dtype=torch.float32)[0], first[b])
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("batch", [33, 48, 49, 64, 65, 130])
+def test_many_rows_of_x(fs, batch, group, zeros):
+    """One pass of every width and several, rows that end inside a tile, columns that end inside a step."""
+    w = _weight(fs, 150 * 16 + 5, 896, group, zeros, seed=batch)
+    x = _x(batch, 896, torch.bfloat16, seed=group)
+    want, bound = _reference(w, x)
+    _check(fs.int4_linear(x, w, out_dtype=torch.float32), want, bound)
+    fs.check_status()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128, 384])
+def test_same_bits_in_every_larger_batch(fs, group):
+    w = _weight(fs, 2601, 1152, group, True, seed=group)
+    x = _x(130, 1152, torch.bfloat16)
+    first = fs.int4_linear(x, w, out_dtype=torch.float32)
+    for b in (9, 16, 17, 32, 33, 48, 64, 65, 128):
+        assert torch.equal(fs.int4_linear(x[:b], w, out_dtype=torch.float32), first[:b]), b
+        assert torch.equal(fs.int4_linear(x[130 - b:], w, out_dtype=torch.float32), first[130 - b:]), b
+
+
+@pytest.mark.parametrize("batch", [1, 8, 16, 50])
+def test_zero_points_of_all_bytes(fs, batch):
+    """A zero point is a byte, not a code: fp16 holds 16 z exactly up to 255."""
+    g = torch.Generator(device=_dev()).manual_seed(0)
+    q = torch.randint(0, 16, (256, 512), generator=g, device=_dev(), dtype=torch.uint8)
+    z = torch.arange(256, device=_dev(), dtype=torch.uint8)[:, None].expand(256, 8).contiguous()
+    w = fs.Int4Weight.from_rows(q, torch.full((256, 8), 0.01, device=_dev()).bfloat16(), z)
+    x = _x(batch, 512, torch.bfloat16)
+    _check(fs.int4_linear(x, w, out_dtype=torch.float32), *_reference(w, x))
+
+
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("batch", [2, 24])
+def test_a_row_of_the_weight_anywhere(fs, batch, group):
+    """The two nibbles of a byte are rows of equal standing, and so are the rows of a tile: what a weight's row gives does
+    not depend on where it lies, in a weight so small that its tiles are all split alike.  (Codes in the lowest bits of an fp16 number lost some of their products' bits.)"""
+    w = _weight(fs, 160, 512, group, True, seed=9)
+    q = w.codes()
+    s = w.scales.permute(0, 3, 2, 1).reshape(160, -1)
+    z = w.zeros.permute(0, 3, 2, 1).reshape(160, -1)
+    x = _x(batch, 512, torch.bfloat16)
+    y = fs.int4_linear(x, w, out_dtype=torch.float32)
+    for shift in (1, 4, 8, 16, 77):
+        at = (torch.arange(160, device=_dev()) + shift) % 160
+        moved = fs.Int4Weight.from_rows(q[at].contiguous(), s[at].contiguous(), z[at].contiguous())
+        assert torch.equal(fs.int4_linear(x, moved, out_dtype=torch.float32), y[:, at])
+
+
+@pytest.mark.parametrize("batch", [12, 40])
+def test_larger_batches_on_streams_and_in_graphs(fs, batch):
+    w = _weight(fs, 3000, 1024, 128, True)
+    xs = [_x(batch, 1024, torch.bfloat16, seed=s) for s in range(3)]
+    want = [fs.int4_linear(x, w) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = []
+    for s, x in zip(streams, xs):
+        with torch.cuda.stream(s):
+            got.append([fs.int4_linear(x, w) for _ in range(4)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, e) for ys, e in zip(got, want) for y in ys)
+    static = xs[0].clone()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = fs.int4_linear(static, w)
+        graphs.append((g, y))
+    for x, e in zip(xs, want):
+        static.copy_(x)
+        torch.cuda.synchronize()
+        for (g, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, e) for _, y in graphs)
+    fs.check_status()
 
 
 def test_streams_and_graphs(fs):

@@ -206,6 +206,44 @@ static size_t beam_workspace(int R, int K, int V, int N, int dtype) {
   return parts * N * 8 + parts * 8 + parts * 4;
 }
 
+int reorder_beams_rounded(int K) { return K <= 2 ? 2 : K <= 4 ? 4 : K <= 8 ? 8 : K <= 16 ? 16 : K <= 32 ? 32 : 64; }
+
+// Bytes of a column: what divides the state's address and strides.
+int reorder_vec(const fmms_beam_state_t& s, int K) {
+  unsigned long long bits = reinterpret_cast<uintptr_t>(s.data) | (unsigned long long)s.beam_stride |
+                            (unsigned long long)s.seg_bytes | (unsigned long long)s.step_bytes;
+  for (int o = 0; o < 2; ++o)
+    if (s.outer[o] > 1) bits |= (unsigned long long)s.outer_stride[o];
+  int vec = K > 32 ? 8 : 16;
+  while (bits & (unsigned long long)(vec - 1)) vec >>= 1;
+  return vec;
+}
+
+template <int KM>
+void launch_reorder_vec(const ReorderParams& p, int vec, dim3 grid, cudaStream_t stm) {
+  switch (vec) {
+    case 16:
+      if constexpr (KM <= 32) reorder_kernel<KM, 16><<<grid, kReorderThreads, 0, stm>>>(p);  // 64 beams: columns of at most 8 bytes
+      break;
+    case 8: reorder_kernel<KM, 8><<<grid, kReorderThreads, 0, stm>>>(p); break;
+    case 4: reorder_kernel<KM, 4><<<grid, kReorderThreads, 0, stm>>>(p); break;
+    case 2: reorder_kernel<KM, 2><<<grid, kReorderThreads, 0, stm>>>(p); break;
+    default: reorder_kernel<KM, 1><<<grid, kReorderThreads, 0, stm>>>(p); break;
+  }
+}
+
+int launch_reorder(const ReorderParams& p, int vec, dim3 grid, cudaStream_t stm) {
+  switch (reorder_beams_rounded(p.K)) {
+    case 2: launch_reorder_vec<2>(p, vec, grid, stm); break;
+    case 4: launch_reorder_vec<4>(p, vec, grid, stm); break;
+    case 8: launch_reorder_vec<8>(p, vec, grid, stm); break;
+    case 16: launch_reorder_vec<16>(p, vec, grid, stm); break;
+    case 32: launch_reorder_vec<32>(p, vec, grid, stm); break;
+    default: launch_reorder_vec<64>(p, vec, grid, stm); break;
+  }
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+}
+
 }  // namespace fmms
 
 using namespace fmms;
@@ -359,65 +397,52 @@ int fmms_reorder_beams(const fmms_beam_state_t* states, int n_states, const void
     const fmms_beam_state_t& s = states[i];
     if (!s.data || s.outer[0] <= 0 || s.outer[1] <= 0 || s.seg_bytes <= 0 || s.step_bytes < 0) return FMMS_ERR_BAD_ARG;
     if (s.step_bytes && s.seg_bytes % s.step_bytes) return FMMS_ERR_BAD_ARG;
+    const long long unit = kReorderThreads, cols = s.seg_bytes / reorder_vec(s, K);
+    if (min(R, kReorderMaxRequests) * ((cols + unit - 1) / unit) >= (1ll << 31)) return FMMS_ERR_UNSUPPORTED;
   }
   int dev = 0, num_sms = 0;
   const int rc = decode_num_sms(&dev, &num_sms);
   if (rc != kOk) return rc;
   if (K == 1) return FMMS_OK;  // one beam: its own parent
   cudaStream_t stm = reinterpret_cast<cudaStream_t>(stream);
-  for (int r0 = 0; r0 < R; r0 += kReorderMaxRequests) {
-    for (int i0 = 0; i0 < n_states; i0 += kReorderMaxStates) {
-      const int n = min(kReorderMaxStates, n_states - i0), nr = min(kReorderMaxRequests, R - r0);
+  // a launch for every width of columns that occurs (rarely more than one), so that each needs no more registers than its own
+  for (int vec = K > 32 ? 8 : 16; vec >= 1; vec >>= 1)
+    for (int r0 = 0; r0 < R; r0 += kReorderMaxRequests) {
       ReorderParams p;
       p.parents = reinterpret_cast<const uint8_t*>(parents) + (size_t)r0 * K * parents_bytes;
       p.parents_wide = parents_bytes == 8;
       p.lengths = lengths ? lengths + r0 : nullptr;
-      p.R = nr;
+      p.R = min(kReorderMaxRequests, R - r0);
       p.K = K;
+      int n = 0;
       long long most = 1;  // units of the largest tensor
-      const int U = K <= 4 ? 4 : K <= 8 ? 2 : 1;
-      for (int i = 0; i < n; ++i) {
-        const fmms_beam_state_t& s = states[i0 + i];
-        ReorderState& d = p.st[i];
-        d.data = reinterpret_cast<uint8_t*>(s.data) + (long long)r0 * K * s.beam_stride;
-        d.beam_stride = s.beam_stride;
-        d.outer_stride[0] = s.outer_stride[0];
-        d.outer_stride[1] = s.outer_stride[1];
-        d.outer[0] = s.outer[0];
-        d.outer[1] = s.outer[1];
-        d.seg_bytes = s.seg_bytes;
-        d.step_bytes = s.step_bytes;
-        unsigned long long bits = reinterpret_cast<uintptr_t>(s.data) | (unsigned long long)s.beam_stride |
-                                  (unsigned long long)s.seg_bytes | (unsigned long long)s.step_bytes;
-        for (int o = 0; o < 2; ++o)
-          if (s.outer[o] > 1) bits |= (unsigned long long)s.outer_stride[o];
-        int vec = K > 32 ? 8 : 16;
-        while (bits & (unsigned long long)(vec - 1)) vec >>= 1;
-        d.vec = vec;
-        const long long cols = s.seg_bytes / vec, unit = kReorderThreads * U, outers = (long long)s.outer[0] * s.outer[1];
-        if (nr * ((cols + unit - 1) / unit) >= (1ll << 31)) return FMMS_ERR_UNSUPPORTED;
-        const long long units = cols >= unit / 2 ? outers * nr * ((cols + unit - 1) / unit) : (outers * nr * cols + kReorderThreads - 1) / kReorderThreads;
-        if (units > most) most = units;
+      for (int i = 0; i < n_states; ++i) {
+        const fmms_beam_state_t& s = states[i];
+        if (reorder_vec(s, K) == vec) {
+          ReorderState& d = p.st[n++];
+          d.data = reinterpret_cast<uint8_t*>(s.data) + (long long)r0 * K * s.beam_stride;
+          d.beam_stride = s.beam_stride;
+          d.outer_stride[0] = s.outer_stride[0];
+          d.outer_stride[1] = s.outer_stride[1];
+          d.outer[0] = s.outer[0];
+          d.outer[1] = s.outer[1];
+          d.seg_bytes = s.seg_bytes;
+          d.step_bytes = s.step_bytes;
+          const long long cols = s.seg_bytes / vec, unit = kReorderThreads * reorder_columns_each(reorder_beams_rounded(K), vec);
+          const long long outers = (long long)s.outer[0] * s.outer[1];
+          const long long units = cols >= unit / 2 ? outers * p.R * ((cols + unit - 1) / unit) : (outers * p.R * cols + kReorderThreads - 1) / kReorderThreads;
+          if (units > most) most = units;
+        }
+        if (n == kReorderMaxStates || (n > 0 && i == n_states - 1)) {
+          // CTAs: enough to fill the GPU eight times over all tensors together, not more than a tensor has work for
+          const long long per = min(((long long)num_sms * 8 + n - 1) / n, most);
+          const int rc_launch = launch_reorder(p, vec, dim3((unsigned)per, (unsigned)n), stm);
+          if (rc_launch != kOk) return rc_launch;
+          n = 0;
+          most = 1;
+        }
       }
-      // CTAs: enough to fill the GPU eight times over all tensors together, not more than a tensor has work for
-      long long per = ((long long)num_sms * 8 + n - 1) / n;
-      if (per > most) per = most;
-      const dim3 grid((unsigned)per, (unsigned)n);
-      if (K <= 2)
-        reorder_kernel<2, 4><<<grid, kReorderThreads, 0, stm>>>(p);
-      else if (K <= 4)
-        reorder_kernel<4, 4><<<grid, kReorderThreads, 0, stm>>>(p);
-      else if (K <= 8)
-        reorder_kernel<8, 2><<<grid, kReorderThreads, 0, stm>>>(p);
-      else if (K <= 16)
-        reorder_kernel<16, 1><<<grid, kReorderThreads, 0, stm>>>(p);
-      else if (K <= 32)
-        reorder_kernel<32, 1><<<grid, kReorderThreads, 0, stm>>>(p);
-      else
-        reorder_kernel<64, 1><<<grid, kReorderThreads, 0, stm>>>(p);
-      if (cudaGetLastError() != cudaSuccess) return kErrCuda;
     }
-  }
   return FMMS_OK;
 }
 

@@ -6,6 +6,10 @@
 // (unless another one takes it) nor written, and nothing is copied back.  It needs no buffer and no order between
 // threads: a thread owns one column (up to 16 bytes at one offset of all K beams of a request), reads it for every beam
 // that changes, and only then writes.  Positions at or behind a request's length are neither read nor written.
+//
+// Bound by HBM: keys and values of 64 x 8 x 2048 x 64 bf16 for eight requests of four beams, half of the positions live: 376 us.
+// A read and a write of what moves at the rate of a plain copy would take 442 us for the worst parents and 320 us for those
+// that were drawn.  Small states cost a launch, 2.3 us.
 #pragma once
 
 #include "fmms_common.cuh"
@@ -24,7 +28,6 @@ struct ReorderState {
   int outer[2];
   long long seg_bytes;        // contiguous bytes of a beam at one outer index
   long long step_bytes;       // bytes of one position, 0: the state has no positions
-  int vec;                    // bytes of a column: divides all of the above and the address
 };
 
 struct ReorderParams {
@@ -55,11 +58,19 @@ __device__ __forceinline__ int reorder_parent(const ReorderParams& p, int r, int
   return (v < 0 || v >= p.K) ? j : (int)v;  // not a beam of the request: keep the own state
 }
 
-// The columns of one tensor.  KM: beams rounded up; U: columns a thread handles at a time.
-template <int KM, int U, int VEC>
+// Columns that a thread handles at a time when a request has up to KM beams (a power of two).  Narrow ones twice as many, or
+// too little is in flight (five beams of 5 x 777 x 123 odd bf16 with half of the positions live: 21 us -> 11 us, together with
+// a kernel of its own for every width, whose registers then are its own: 64 instead of 108).
+__host__ __device__ constexpr int reorder_columns_each(int KM, int vec) {
+  const int few = KM <= 4 ? 4 : KM <= 8 ? 2 : 1;
+  return vec <= 4 && KM <= 8 ? 2 * few : few;
+}
+
+// The columns of one tensor.  KM: beams rounded up.
+template <int KM, int VEC>
 __device__ __forceinline__ void reorder_columns(const ReorderParams& p, const ReorderState& s, const int* prefix) {
   using V = typename ReorderVec<VEC>::type;
-  constexpr int kUnit = kReorderThreads * U;
+  constexpr int U = reorder_columns_each(KM, VEC), kUnit = kReorderThreads * U;
   const int tid = threadIdx.x;
   const long long cols = s.seg_bytes / VEC;
   const long long outers = (long long)s.outer[0] * s.outer[1];
@@ -130,17 +141,17 @@ __device__ __forceinline__ void reorder_columns(const ReorderParams& p, const Re
   }
 }
 
-// grid (CTAs per tensor, tensors)
-template <int KM, int U>
+// grid (CTAs per tensor, tensors); VEC: bytes of a column in all of them
+template <int KM, int VEC>
 __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_constant__ ReorderParams p) {
   __shared__ int prefix[kReorderMaxRequests + 1];
   const ReorderState& s = p.st[blockIdx.y];
-  constexpr int kUnit = kReorderThreads * U;
-  if (s.seg_bytes / s.vec >= kUnit / 2) {
+  constexpr int kUnit = kReorderThreads * reorder_columns_each(KM, VEC);
+  if (s.seg_bytes / VEC >= kUnit / 2) {
     for (int r = threadIdx.x; r < p.R; r += kReorderThreads) {
       long long live = s.seg_bytes;
       if (p.lengths && s.step_bytes) live = min(live, max(0, p.lengths[r]) * s.step_bytes);
-      prefix[r + 1] = (int)((live / s.vec + kUnit - 1) / kUnit);
+      prefix[r + 1] = (int)((live / VEC + kUnit - 1) / kUnit);
     }
     __syncthreads();
     if (threadIdx.x < 32) {  // inclusive sums, 32 at a time
@@ -161,15 +172,7 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
     }
     __syncthreads();
   }
-  switch (s.vec) {
-    case 16:
-      if constexpr (KM <= 32) reorder_columns<KM, U, 16>(p, s, prefix);  // 64 beams: columns of at most 8 bytes
-      break;
-    case 8: reorder_columns<KM, U, 8>(p, s, prefix); break;
-    case 4: reorder_columns<KM, U, 4>(p, s, prefix); break;
-    case 2: reorder_columns<KM, U, 2>(p, s, prefix); break;
-    default: reorder_columns<KM, U, 1>(p, s, prefix); break;
-  }
+  reorder_columns<KM, VEC>(p, s, prefix);
 }
 
 }  // namespace fmms

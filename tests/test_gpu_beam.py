@@ -474,3 +474,17 @@ def test_search_step_in_a_graph(fs):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, eager)) and _same(cache, after)
+
+
+def test_reorder_states_of_every_width_at_once(fs):
+    """Columns of 1, 2, 4, 8 and 16 bytes in one call, more than one launch's worth of one width among them."""
+    g = torch.Generator(device=_dev()).manual_seed(11)
+    r, k = 5, 6
+    parents = torch.randint(0, k, (r, k), generator=g, device=_dev())
+    shapes = [((r * k, 7), torch.uint8), ((r * k, 9), torch.bfloat16), ((r * k, 333, 3), torch.float32), ((r * k, 1), torch.int64),
+              ((r * k, 40, 64), torch.bfloat16)] + [((r * k, 16 + i), torch.bfloat16) for i in range(130)]
+    states = [torch.randint(0, 100, s, generator=g, device=_dev()).to(t) for s, t in shapes]
+    at = (torch.arange(r, device=_dev())[:, None] * k + parents).view(-1)
+    want = [s[at] for s in states]
+    fs.reorder_beams(states, parents)
+    assert all(torch.equal(s, w) for s, w in zip(states, want))

@@ -7,9 +7,9 @@
 // threads: a thread owns one column (up to 16 bytes at one offset of all K beams of a request), reads it for every beam
 // that changes, and only then writes.  Positions at or behind a request's length are neither read nor written.
 //
-// Bound by HBM: keys and values of 64 x 8 x 2048 x 64 bf16 for eight requests of four beams, half of the positions live: 376 us.
-// A read and a write of what moves at the rate of a plain copy would take 442 us for the worst parents and 320 us for those
-// that were drawn.  Small states cost a launch, 2.3 us.
+// Bound by HBM: keys and values of 64 x 8 x 2048 x 64 bf16 for eight requests of four beams, half of the positions live: 376 us
+// a call over three draws of parents and lengths, whose reads and writes (2.27 GB) take 352 us at the rate of a plain copy.
+// Small states cost a launch, 2.3 us.
 #pragma once
 
 #include "fmms_common.cuh"

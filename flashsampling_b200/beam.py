@@ -183,8 +183,8 @@ def reorder_beams(
     """Beam ``j`` of request ``r`` continues beam ``parents[r, j]``: in every state, in place,
     ``state[.., r * beams + j, ..] = state[.., r * beams + parents[r, j], ..]``, all beams at once.
 
-    Without ``lengths`` whole beams move.  With ``lengths`` only the first ``lengths[r]`` positions along ``length_dim`` move; what lies behind them stays as it
-    is (lengths beyond the dimension count as all of it).  A parent outside ``0..beams-1`` keeps the beam's own state.
+    Without ``lengths`` whole beams move.  With ``lengths`` only the first ``lengths[r]`` positions along ``length_dim`` do;
+    what lies behind them stays as it is (lengths beyond the dimension count as all of it).  A parent outside ``0..beams-1`` keeps the beam's own state.
     One launch for up to 64 tensors; a beam that keeps its own state costs no traffic.  Up to 64 beams.  States may
     be strided views as long as they do not overlap, themselves or one another."""
     states = [states] if isinstance(states, torch.Tensor) else list(states)
@@ -302,8 +302,8 @@ class BeamSearch:
         return BeamStep(out.scores, tokens, out.parents)
 
     def done(self) -> bool:
-        """Whether every beam is finished (waits for the GPU)."""
-        return bool(self.finished.all())
+        """Whether every beam is finished or has run out of tokens that may follow (waits for the GPU)."""
+        return bool((self.finished | (self.scores == -math.inf)).all())
 
     def best(self, length_penalty: float = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
         """``(tokens [requests, steps], scores [requests])`` of every request's best hypothesis by score divided by

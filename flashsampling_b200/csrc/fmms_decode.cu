@@ -283,6 +283,7 @@ int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void*
   else
     rc = int4_plan(pl, D, group);
   if (rc != kOk) return rc;
+  if (mma && mp.passes > 65535) return FMMS_ERR_UNSUPPORTED;  // two to four million rows of x
   const size_t need = mma ? int4_mma_workspace(D, B, group) : int4_workspace(pl, V);
   if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need)) return FMMS_ERR_WORKSPACE;
   int dev = 0, num_sms = 0;

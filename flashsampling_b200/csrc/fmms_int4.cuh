@@ -330,10 +330,6 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_linear_kernel(const I
       __syncthreads();
     }
 
-    float down[2];  // from the units of the sums to the result
-#pragma unroll
-    for (int i = 0; i < 2; ++i) down[i] = t * 2 + i < nb ? pow2(-row_exp[t * 2 + i]) : 0.f;
-
     clear();
     for (int pr = p_first; pr <= p_last && begin < end; ++pr) {
       int u, hi;
@@ -417,10 +413,17 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_linear_kernel(const I
       }
       // the warp's part of this pair in this phase is complete
       const bool has_start = begin <= pr * p.units, has_end = end >= (pr + 1) * p.units;
+      // From the units of the sums to the result, by 2^(20 - exponent) in two halves: no step of it lies beyond both ends.
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+      for (int i = 0; i < 2; ++i) {
+        const int e = t * 2 + i < nb ? 20 - row_exp[t * 2 + i] : 0;
+        const float down0 = pow2(e >> 1), down1 = pow2(e - (e >> 1));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) tot[m][j] = tot[m][j] * 0x1p20f * down[j & 1];
+        for (int m = 0; m < 2; ++m) {
+          tot[m][i] = tot[m][i] * down0 * down1;
+          tot[m][2 + i] = tot[m][2 + i] * down0 * down1;
+        }
+      }
       if (!has_start) {
         float* mine = pieces + warp * (2 * 128) + lane;
 #pragma unroll

@@ -398,10 +398,10 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
     const int r16 = lane & 15, tile_of = lane >> 4;  // row within its tile; first or second tile
     const int place = (r16 & 7) * 2 + (r16 >> 3);    // within the 16 scales of a group
     const int nb = min(NC, q.B - pass * p.n);
-    // what brings column first_col + lane back to its row of x
-    float down = 0.f;
-    if (lane < kCols && first_col + lane < nb)
-      down = __uint_as_float((uint32_t)(127 - p.exponents[pass * kInt4MmaPass + first_col + lane]) << 23);
+    // what brings column first_col + lane back to its row of x, in two halves: no step of it lies beyond both ends
+    int e = 0;
+    if (lane < kCols && first_col + lane < nb) e = 20 - p.exponents[pass * kInt4MmaPass + first_col + lane];
+    const float down0 = __uint_as_float((uint32_t)(127 + (e >> 1)) << 23), down1 = __uint_as_float((uint32_t)(127 + e - (e >> 1)) << 23);
     int slot = 0, d = 0, dround = 0;
 #pragma unroll 1
     for (int block = 0; block < blocks; ++block) {
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
       const int v = (t_begin + block * 8 + quad + tile_of * 4) * kInt4Tile + r16;
 #pragma unroll
       for (int i = 0; i < kCols; ++i) {
-        const float y = ((i & 1) ? tot[i / 2].y : tot[i / 2].x) * 0x1p20f * __shfl_sync(0xffffffffu, down, i);
+        const float y = ((i & 1) ? tot[i / 2].y : tot[i / 2].x) * __shfl_sync(0xffffffffu, down0, i) * __shfl_sync(0xffffffffu, down1, i);
         if (there && v < q.V && first_col + i < nb) int4_store(q, pass * p.n + first_col + i, v, y);
       }
     }

@@ -27,6 +27,7 @@ class Int4Weight:
     ``16 tile + 8 + g`` (high nibble) of column ``64 chunk + 16 j + 8 b0 + 2 t + b1``.  ``scales`` (bf16 or fp16) and
     ``zeros`` (uint8, or ``None``: 8 everywhere) are ``[tiles, groups, 8, 2]``, row ``g`` and row ``8 + g`` next to
     each other.  A weight is ``(q - zero) * scale``.  What rows and columns beyond the weight hold does not matter.
+    The tensors' contents may change, the tensors themselves may not.
 
     ``Int4Weight.from_rows`` lays out plain codes, ``Int4Weight.quantize`` rounds a floating-point weight.
     """
@@ -50,13 +51,20 @@ class Int4Weight:
         for name, t in (("qweight", qweight), ("scales", scales), ("zeros", zeros)):
             if t is not None and (not t.is_contiguous() or t.data_ptr() % 16 or t.device != qweight.device):
                 raise ValueError(f"{name} must be contiguous, start on a 16-byte boundary and lie on qweight's device")
-        self.qweight, self.scales, self.zeros = qweight, scales, zeros
-        self.rows, self.cols, self.group_size = int(rows), int(cols), cols // scales.shape[1]
-        # what every call passes on: the tensors above are kept, so their addresses stay
-        self._args = (
+        rows, cols, group = int(rows), int(cols), cols // scales.shape[1]
+        # what every call passes on: the tensors are kept and no attribute changes, so their addresses stay
+        args = (
             qweight.data_ptr(), scales.data_ptr(), _DTYPES[scales.dtype], zeros.data_ptr() if zeros is not None else None,
-            self.rows, self.cols, self.group_size,
+            rows, cols, group,
         )
+        for name, value in zip(self.__slots__, (qweight, scales, zeros, rows, cols, group, args)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError("an Int4Weight keeps its tensors: make a new one")
+
+    def __reduce__(self):
+        return (Int4Weight, (self.qweight, self.scales, self.zeros, self.rows, self.cols))
 
     @property
     def shape(self) -> tuple[int, int]:

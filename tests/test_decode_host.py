@@ -235,3 +235,16 @@ def test_description_refuses():
         beam._describe(torch.zeros(6, 4, 8)[..., ::2], 0, 1, 2, 3, desc, True)
     with pytest.raises(ValueError):  # three uneven dimensions around the beams
         beam._describe(torch.zeros(4, 3, 6, 4, 5)[::2, ::2, :, ::2], 2, None, 2, 3, desc, False)
+
+
+def test_a_weight_keeps_its_tensors():
+    """Calls pass on the addresses that the weight was made with: no attribute may change behind them."""
+    import pickle
+
+    q, s, z = _codes(20, 128, 64, True)
+    w = fs.Int4Weight.from_rows(q, s, z)
+    for name in ("qweight", "scales", "zeros", "rows", "_args"):
+        with pytest.raises(AttributeError):
+            setattr(w, name, None)
+    again = pickle.loads(pickle.dumps(w))
+    assert again.shape == w.shape and torch.equal(again.dequantize(), w.dequantize())

@@ -488,3 +488,13 @@ def test_reorder_states_of_every_width_at_once(fs):
     want = [s[at] for s in states]
     fs.reorder_beams(states, parents)
     assert all(torch.equal(s, w) for s, w in zip(states, want))
+
+
+def test_search_that_runs_out_of_tokens(fs):
+    """A head whose logits are all NaN leaves no token: no beam goes on, and the search is done."""
+    w = torch.full((64, 32), float("nan"), device=_dev(), dtype=torch.bfloat16)
+    weight = fs.Int4Weight.from_rows(torch.zeros(64, 32, dtype=torch.uint8, device=_dev()), w[:, :1].contiguous())
+    search = fs.BeamSearch(weight, 2, 3, 4, eos_token=5)
+    assert not search.done()
+    out = search.step(torch.ones(6, 32, device=_dev(), dtype=torch.bfloat16))
+    assert bool((out.scores == -float("inf")).all()) and search.done()

@@ -229,6 +229,27 @@ def test_same_bits_in_every_larger_batch(fs, group):
         assert torch.equal(fs.int4_linear(x[130 - b:], w, out_dtype=torch.float32), first[130 - b:]), b
 
 
+@pytest.mark.parametrize("cols,group", [(32, 32), (96, 32), (4128, 32), (64, 64), (192, 64), (320, 64), (128, 128), (384, 384)])
+@pytest.mark.parametrize("batch", [10, 64])
+def test_larger_batches_with_half_filled_steps(fs, batch, cols, group):
+    w = _weight(fs, 1200, cols, group, True, seed=cols)
+    x = _x(batch, cols, torch.float16)
+    want, bound = _reference(w, x)
+    _check(fs.int4_linear(x, w, out_dtype=torch.float32), want, bound)
+
+
+@pytest.mark.parametrize("batch", [4, 12])
+def test_scales_far_from_one(fs, batch):
+    """Scales at the ends of bf16 with rows of x at the other: the result is in range, and so is every step to it."""
+    w = _weight(fs, 48, 256, 64, True)
+    x = _x(batch, 256, torch.bfloat16)
+    for up in (110, -60):
+        scaled = fs.Int4Weight(w.qweight, (w.scales.float() * 2.0**up).bfloat16(), w.zeros, w.rows, w.cols)
+        rows = (x.float() * 2.0**-up).bfloat16()
+        want, bound = _reference(scaled, rows)
+        _check(fs.int4_linear(rows, scaled, out_dtype=torch.float32), want, bound)
+
+
 @pytest.mark.parametrize("batch", [1, 8, 16, 50])
 def test_zero_points_of_all_bytes(fs, batch):
     """A zero point is a byte, not a code: fp16 holds 16 z exactly up to 255."""

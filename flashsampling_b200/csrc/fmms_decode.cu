@@ -128,7 +128,7 @@ static void int4_mma_plan(Int4MmaPlan& pl, int D, int B, int group, bool zeros) 
   pl.n = ((B + pl.passes - 1) / pl.passes + 15) / 16 * 16;
   const int units = int4_step_units(gr, pl.n);
   pl.row_steps = ((D + kInt4Unit - 1) / kInt4Unit + units - 1) / units;
-  const int weights = kInt4MmaWeightWarps * kInt4MmaRing * (units * 1024 + (zeros ? 64 : 0));
+  const int weights = kInt4MmaWeightWarps * kInt4MmaRing * (units * 1024 + (zeros ? 128 : 0));
   const int scales = kInt4MmaSumWarps * kInt4MmaScaleRing * int4_step_groups(gr, pl.n) * 64;
   pl.x_stages = min(kInt4MmaMaxX, (kInt4SmemLimit - weights - scales) / int4_x_bytes(pl.n, gr));
   pl.ring_off = pl.x_stages * int4_x_bytes(pl.n, gr);

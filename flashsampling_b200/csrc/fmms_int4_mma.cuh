@@ -3,7 +3,7 @@
 //
 // mma.sync takes eight cycles for a 16 x 16 x 8 product here, so that beyond eight rows the products and not the weight's
 // stream set its pace (151936 x 4096: 55 us for one row, 59 us for 8, 83 us for 16, 216 us for 32, where this kernel takes
-// 89 us and 105 us; 128256 x 8192 at 16 rows: 200 us and 145 us).  tcgen05.mma takes 128 weight
+// 89 us and 106 us; 128256 x 8192 at 16 rows: 200 us and 143 us).  tcgen05.mma takes 128 weight
 // rows against all rows of x at once, and it reads one operand from tensor memory: the weights go from registers there,
 // in the very layout the stored order is made for (tcgen05.st .16x128b places what a lane holds of a 16 x 16 operand), and
 // never through shared memory as fp16.
@@ -17,7 +17,8 @@
 //   warp 24      issues the products, a group of columns to an accumulator
 //   warp 25      fetches x, a bulk copy per step
 // The zero points are products as well: behind the columns of a group come 16 more, of which three hold z on the one side
-// and minus the sum of x over the group, cut into three fp16 parts, on the other.  That halves what the reading back
+// and minus the sum of x over the group, cut into three fp16 parts, on the other (the z of all groups of a step, up to four,
+// lie in one such operand, at columns 4 g.., and the sums of group g meet only those).  That halves what the reading back
 // costs (a multiply-add per row of x and group instead of two and a load).
 // int4_stage_x writes x beforehand, as fp16 in the swizzled layout of the products with those columns behind every step.
 // Its power of two per row puts the row's largest element into [2^7, 2^8), so that a group's sum fits fp16 as well; what lies
@@ -36,14 +37,19 @@ constexpr int kInt4MmaWeightWarps = 16, kInt4MmaSumWarps = 8;
 constexpr int kInt4MmaThreads = (kInt4MmaWeightWarps + kInt4MmaSumWarps + 2) * 32;
 constexpr int kInt4MmaPass = 64;       // rows of x in a pass, at most
 constexpr int kInt4MmaRing = 4;        // steps in a warp's ring (every second one is its own)
-constexpr int kInt4MmaSlots = 2;       // steps in tensor memory
 constexpr int kInt4MmaMaxX = 6;        // steps of x in shared memory
 constexpr int kInt4MmaScaleRing = 8;   // steps of scales
 // A step is what changes hands at a time: 256 columns, for barriers, not arithmetic, set the pace of a shorter one; 128 where
-// tensor memory (two slots of operands at 64 columns a unit, with zeros 8 more a group, and of accumulators at a column per
-// row of x and group) does not hold two of them.
+// tensor memory (of a slot: operands at 64 columns a unit, zero points 8, accumulators at a column per row of x and group)
+// does not hold two of them.
 __host__ __device__ constexpr int int4_step_units(int group, int n) { return group < kInt4Unit || n > 48 ? 1 : 2; }
 __host__ __device__ constexpr int int4_step_groups(int group, int n) { return int4_step_units(group, n) * int4_unit_groups(group); }
+// Steps in tensor memory.  Three let a weight warp fill while the products of the step before still run; with two it waits for
+// them (128256 x 8192 at 16 rows: 147 us, with three 143 us).
+__host__ __device__ constexpr int int4_slots(int group, int n) {
+  const int fit = kTmemCols / (int4_step_units(group, n) * 64 + 8 + int4_step_groups(group, n) * n);
+  return fit < 3 ? fit : 3;
+}
 __host__ __device__ constexpr int int4_mma_max_n(int group) { return group == 32 ? 32 : kInt4MmaPass; }
 __host__ __device__ constexpr int int4_x_bytes(int n, int group) { return (int4_step_units(group, n) * 2 + 1) * n * 128; }  // of a step
 
@@ -123,10 +129,11 @@ __global__ void __launch_bounds__(256) int4_stage_x_kernel(const Int4MmaParams p
       // minus the sum, in three parts
       const __half h0 = __float2half_rn(-s), h1 = __float2half_rn(-s - __half2float(h0));
       const __half h2 = __float2half_rn(-s - __half2float(h0) - __half2float(h1));
-      const int c16 = in_step / GR * 2;
-      *reinterpret_cast<uint4*>(dst + place(step_units * 2, c16)) =
-          make_uint4((uint32_t)__half_as_ushort(h0) | ((uint32_t)__half_as_ushort(h1) << 16), (uint32_t)__half_as_ushort(h2), 0u, 0u);
-      *reinterpret_cast<uint4*>(dst + place(step_units * 2, c16 + 1)) = make_uint4(0u, 0u, 0u, 0u);
+      const int gi = in_step / GR;
+      const uint32_t w0 = (uint32_t)__half_as_ushort(h0) | ((uint32_t)__half_as_ushort(h1) << 16), w1 = (uint32_t)__half_as_ushort(h2);
+      const uint4 parts = gi & 1 ? make_uint4(0u, 0u, w0, w1) : make_uint4(w0, w1, 0u, 0u), none = make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(dst + place(step_units * 2, gi * 2)) = gi < 2 ? parts : none;
+      *reinterpret_cast<uint4*>(dst + place(step_units * 2, gi * 2 + 1)) = gi < 2 ? none : parts;
     }
   }
 }
@@ -179,8 +186,8 @@ __device__ __forceinline__ void tmem_load8(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ void tmem_store_zero_points(uint32_t taddr, uint32_t a0, uint32_t a1) {
-  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a0), "r"(a1), "r"(0u), "r"(0u) : "memory");
+__device__ __forceinline__ void tmem_store_zero_points(uint32_t taddr, const uint32_t (&a)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]) : "memory");
 }
 
 // A in tensor memory, B in shared memory
@@ -220,13 +227,13 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
   constexpr int kGroups = int4_unit_groups(GR), kSteps = GR / 16;
   constexpr int kStepU = int4_step_units(GR, NC), kStepG = int4_step_groups(GR, NC);
   constexpr int kXBytes = int4_x_bytes(NC, GR);
-  // tensor memory: operands of both slots, zero points (of both slots, or one for all), accumulators of both slots
-  constexpr int kZeroCols = ZP ? kStepG * 8 : 0;
-  constexpr int kZeroAt = kInt4MmaSlots * kStepU * 64, kSumAt = kZeroAt + (ZP ? kInt4MmaSlots * kZeroCols : 8);
-  static_assert(kSumAt + kInt4MmaSlots * kStepG * NC <= kTmemCols, "tensor memory");
+  // tensor memory: operands of all slots, zero points (of each slot, or one for all), accumulators of all slots
+  constexpr int kSlots = int4_slots(GR, NC), kZeroCols = ZP ? 8 : 0;
+  constexpr int kZeroAt = kSlots * kStepU * 64, kSumAt = kZeroAt + (ZP ? kSlots * kZeroCols : 8);
+  static_assert(kSlots >= 2 && kStepG <= 4 && kSumAt + kSlots * kStepG * NC <= kTmemCols, "tensor memory");
   constexpr int kScaleBytes = kStepG * 64;  // of a step, for the two tiles of a warp
   constexpr int kScaleCopy = kStepG == 4 ? 8 : 4, kScaleLanes = kStepG * 32 / kScaleCopy;
-  __shared__ uint64_t a_full[kInt4MmaSlots], done[kInt4MmaSlots], d_empty[kInt4MmaSlots];
+  __shared__ uint64_t a_full[kSlots], done[kSlots], d_empty[kSlots];
   __shared__ uint64_t x_full[kInt4MmaMaxX], x_empty[kInt4MmaMaxX];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_word;
@@ -241,7 +248,7 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
   const int blocks = (t_count + 7) / 8, row_steps = p.row_steps, steps = blocks * row_steps;
 
   if (tid == 0) {
-    for (int i = 0; i < kInt4MmaSlots; ++i) {
+    for (int i = 0; i < kSlots; ++i) {
       mbar_init(&a_full[i], kInt4MmaWeightWarps / 2);
       mbar_init(&done[i], 1);  // the products: operands free, sums there
       mbar_init(&d_empty[i], kInt4MmaSumWarps);
@@ -264,14 +271,14 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
 
   if (warp < kInt4MmaWeightWarps) {
     // ------------------------------ weights ------------------------------
-    const int half = (warp >> 2) & 1, a = warp >> 3;  // chunk of every unit; steps a, a + 2, .., all in slot a
+    const int half = (warp >> 2) & 1, a = warp >> 3;  // chunk of every unit; steps a, a + 2, ..
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    // zeros: this half's groups of a step, half and half + 2, 16 bytes for each of the two tiles
-    constexpr int kZeroGroups = ZP ? (kStepG + 1) / 2 : 0;
-    constexpr int kSlot = kStepU * 1024 + (ZP ? 64 : 0);  // bytes of a step: two tiles, one chunk of each unit; zeros
+    constexpr int kSlot = kStepU * 1024 + (ZP ? 128 : 0);  // bytes of a step: two tiles, one chunk of each unit; zeros
     uint8_t* ring = smem + p.ring_off + warp * (kInt4MmaRing * kSlot);
     const uint32_t ring_at = smem_u32(ring);
-    const int z_tile = lane >> 2 & 1, z_group = half + 2 * (lane >> 3);  // lanes below 8 kZeroGroups copy 4 bytes of these
+    // zeros: the warps of the first half have those of all groups of the step, 16 bytes for each of the two tiles
+    const bool zeros_too = ZP && half == 0;
+    const int z_tile = lane >> 2 & 1, z_group = lane >> 3;  // lanes below 8 kStepG copy 4 bytes of these
     const long long four = (long long)q.chunks * (4 * 512);  // four tiles on
     int f_block = 0, f_step = a - 2, f_slot = 0;
     const uint8_t *f_q = nullptr, *f_z = nullptr;
@@ -304,7 +311,7 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
         if constexpr (ZP) {
           // groups of more than one unit repeat
           const int gr = GR == kInt4Unit ? (q.group_units == 1 ? unit + z_group : (unit + z_group) / q.group_units) : unit * kGroups + z_group;
-          if (lane < 8 * kZeroGroups && z_group < kStepG && left > z_tile * 4 && gr < q.groups)
+          if (zeros_too && z_group < kStepG && left > z_tile * 4 && gr < q.groups)
             copy_async<4>(dst + kStepU * 1024 + lane * 4, f_z + gr * 16);
         }
         f_q += 2 * kStepU * 1024;
@@ -314,51 +321,61 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
     };
 #pragma unroll 1
     for (int i = 0; i < kInt4MmaRing - 1; ++i) fetch();
-    // z 2^-20 at columns 0, 1 and 2 of a row: what lane (g, t) holds of the operand, for rows g and 8 + g.  Above 127 that is
-    // no subnormal: the number's step doubles at 2^-13.
-    const int t = lane & 3;
-    const uint32_t z_mask = t == 0 ? 0xffffffffu : t == 1 ? 0x0000ffffu : 0u;
+    // z 2^-20 of group g at columns 4 g, 4 g + 1 and 4 g + 2 of a row: what lane (row, t) holds of the operand for rows `row`
+    // and 8 + row is that of group t / 2, and 8 columns on of group 2 + t / 2.  Above 127 that is no subnormal: the number's
+    // step doubles at 2^-13.
+    const uint32_t z_mask = lane & 1 ? 0x0000ffffu : 0xffffffffu;
+    const int z_mine = lane >> 1 & 1;
     auto zero_point = [&](uint32_t z) { return min(z << 4, (z << 3) + 1024u) * 0x00010001u & z_mask; };
-    auto store_zero_points = [&](uint32_t at, uint32_t pair) { tmem_store_zero_points(at, zero_point(pair & 0xffu), zero_point(pair >> 8)); };
     if constexpr (!ZP)
       if (warp < 4) {  // before this warp's first step, and read from step 0 on, which is its own
-        store_zero_points(tmem + lanes + kZeroAt, 0x0808u);
-        store_zero_points(tmem + lanes + (16u << 16) + kZeroAt, 0x0808u);
+        const uint32_t eight = zero_point(8), all[4] = {eight, eight, eight, eight};
+        tmem_store_zero_points(tmem + lanes + kZeroAt, all);
+        tmem_store_zero_points(tmem + lanes + (16u << 16) + kZeroAt, all);
       }
-    int slot = 0, round = 0, block = 0, step = a - 2;
+    int slot = 0, at_slot = a, round = 0, block = 0, step = a - 2;  // at_slot, round: where the step goes, for the how manieth time
 #pragma unroll 1
-    for (;; ++round) {
+    for (;;) {
       next(block, step);
       if (block >= blocks) break;
       const int mine = t_count - block * 8 - quad;  // > 0: the first tile is there, > 4: the second too
       asm volatile("cp.async.wait_group %0;" ::"n"(kInt4MmaRing - 2) : "memory");
       if constexpr (ZP) __syncwarp();  // zeros were copied by other lanes
       const uint8_t* src = ring + slot * kSlot;
-      if (round > 0) mbar_wait(&done[a], (uint32_t)(round - 1) & 1u, abort_flag, p.status_dev);
+      if (round > 0) mbar_wait(&done[at_slot], (uint32_t)(round - 1) & 1u, abort_flag, p.status_dev);
       tc_fence_after();
-      const uint32_t at = tmem + lanes + a * (kStepU * 64) + half * 32;
+      const uint32_t at = tmem + lanes + at_slot * (kStepU * 64) + half * 32;
 #pragma unroll
       for (int i = 0; i < kStepU; ++i)
 #pragma unroll
         for (int m = 0; m < 2; ++m)
           if (mine > m * 4) tmem_store_codes(at + ((uint32_t)(m * 16) << 16) + i * 64, *reinterpret_cast<const uint4*>(src + i * 1024 + m * 512 + lane * 16));
-      if constexpr (ZP) {
+      if (zeros_too) {
 #pragma unroll
-        for (int j = 0; j < kZeroGroups; ++j)
+        for (int m = 0; m < 2; ++m) {
+          uint32_t z[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            if (half + 2 * j >= kStepG) continue;
-            const uint32_t pair = *reinterpret_cast<const uint16_t*>(src + kStepU * 1024 + (j * 2 + m) * 16 + (lane >> 2) * 2);
-            store_zero_points(tmem + lanes + ((uint32_t)(m * 16) << 16) + kZeroAt + a * kZeroCols + (half + 2 * j) * 8, pair);
+          for (int j = 0; j < kStepG; j += 2) {
+            // (a step of one group has no second one: what is read in its place meets zeros of x)
+            const uint32_t pair = *reinterpret_cast<const uint16_t*>(src + kStepU * 1024 + ((j + z_mine) * 2 + m) * 16 + (lane >> 2) * 2);
+            z[j] = zero_point(pair & 0xffu);
+            z[j + 1] = zero_point(pair >> 8);
           }
+          tmem_store_zero_points(tmem + lanes + ((uint32_t)(m * 16) << 16) + kZeroAt + at_slot * kZeroCols, z);
+        }
         __syncwarp();  // everybody has read the slot's zeros
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&a_full[a]);
+      if (lane == 0) mbar_arrive(&a_full[at_slot]);
       fetch();
       if (++slot == kInt4MmaRing) slot = 0;
+      at_slot += 2;
+      if (at_slot >= kSlots) {
+        at_slot -= kSlots;
+        ++round;
+      }
     }
   } else if (warp < kInt4MmaWeightWarps + kInt4MmaSumWarps) {
     // ------------------------------ sums ------------------------------
@@ -439,7 +456,7 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&d_empty[d]);
-        if (++d == kInt4MmaSlots) {
+        if (++d == kSlots) {
           d = 0;
           ++dround;
         }
@@ -472,7 +489,7 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
         for (int gi = 0; gi < kStepG; ++gi) {
           if (gi >= groups) break;
           const uint64_t dz = desc + (uint64_t)(kStepU * 2 * (NC * 128 / 16) + gi * 2);
-          umma_f16_ts(td + gi * NC, tz + (ZP ? gi * 8 : 0), dz, p.idesc, 0u);
+          umma_f16_ts(td + gi * NC, tz, dz, p.idesc, 0u);
 #pragma unroll
           for (int j = 0; j < kSteps; ++j) {
             const int k = gi * kSteps + j;  // 16 columns: eight of tensor memory, 32 bytes of each row of x
@@ -483,7 +500,7 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
         umma_commit(&x_empty[x]);
       }
       __syncwarp();
-      if (++a == kInt4MmaSlots) {
+      if (++a == kSlots) {
         a = 0;
         ++around;
       }

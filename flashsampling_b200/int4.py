@@ -199,4 +199,5 @@ def _launch(x, stride, weight, b, out, out_stride, index):
     return _lib.load().fmms_int4_linear(
         x.data_ptr(), _DTYPES[x.dtype], stride, qw, scales, scale_dtype, zeros, rows, cols, group, b,
         out.data_ptr(), _DTYPES[out.dtype], out_stride, ws.data_ptr() if nbytes else None, nbytes,
-        _status_word(x.device).data_ptr(), torch._C._cuda_getCurrentRawStream(index))
+        _status_word(x.device).data_ptr() if b > 8 else None,  # up to eight rows: no waits between warps
+        torch._C._cuda_getCurrentRawStream(index))

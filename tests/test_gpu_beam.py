@@ -498,3 +498,41 @@ def test_search_that_runs_out_of_tokens(fs):
     assert not search.done()
     out = search.step(torch.ones(6, 32, device=_dev(), dtype=torch.bfloat16))
     assert bool((out.scores == -float("inf")).all()) and search.done()
+
+
+_CAPTURED_FIRST = """
+import torch
+import flashsampling_b200 as fs
+dev = torch.device("cuda", 0)
+g = torch.Generator().manual_seed(0)
+q = torch.randint(0, 16, (300, 256), generator=g, dtype=torch.uint8).to(dev)
+w = fs.Int4Weight.from_rows(q, torch.full((300, 2), 0.01, device=dev).bfloat16())
+h = torch.randn(4, 256, generator=g).bfloat16().to(dev)
+many = torch.randn(20, 256, generator=g).bfloat16().to(dev)
+scores = torch.zeros(1, 4, device=dev)
+state = torch.arange(4 * 5, device=dev).view(4, 5)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    logits = fs.int4_linear(h, w, out_dtype=torch.float32)
+    more = fs.int4_linear(many, w, out_dtype=torch.float32)
+    step = fs.beam_search_step(logits, scores)
+    fs.reorder_beams(state, step.parents)
+graph.replay()
+torch.cuda.synchronize()
+eager = fs.beam_search_step(fs.int4_linear(h, w, out_dtype=torch.float32), scores)
+assert torch.equal(eager.tokens, step.tokens) and torch.equal(eager.parents, step.parents) and torch.equal(eager.scores, step.scores)
+assert torch.equal(more, fs.int4_linear(many, w, out_dtype=torch.float32))
+assert torch.equal(state, torch.arange(4 * 5, device=dev).view(4, 5)[step.parents[0]])
+fs.check_status()
+print("captured first")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture(fs):
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", _CAPTURED_FIRST], cwd=root, capture_output=True, text=True, timeout=240)
+    assert done.returncode == 0 and "captured first" in done.stdout, done.stderr[-2000:]

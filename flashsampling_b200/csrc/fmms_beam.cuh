@@ -206,7 +206,9 @@ __global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamPa
     if (v_begin + i * kBeamThreads + tid < v_end) m = fmaxf(m, beam_vec_max<T>(ring[i / 2][i % 2][tid]));
   // The N-th largest of 32 groups' maxima (8 lanes each; up to 32 candidates), or of 128 (2 lanes): into sh_pivot; the
   // largest: returned.
-  const bool wide = p.N <= 32;
+  // Few vectors leave groups of 8 lanes empty, and the bound would be -inf (64 x 12 x 1500 bf16, 24
+  // candidates: 26 us, and 15 us with groups of 2).
+  const bool wide = p.N <= 32 && v_end - v_begin >= kBeamThreads;
   auto bound = [&](float m) {
     float gm = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     if (wide) {
@@ -433,9 +435,12 @@ __device__ __forceinline__ bool beam_before(double t1, unsigned int a1, double t
   return t1 > t2 || (t1 == t2 && a1 < a2);
 }
 
-// One CTA per request.  What the slices kept is a set of lists, K * splits of them with N entries each.  Up to 1024
-// entries at a time, joined with the best N of the ones before, shrink to what reaches their bound (again and again
-// while they are many) and are counted against each other.
+// One CTA per request.  What the slices kept is a set of lists, K * splits of them with N entries each in descending order.
+// Many lists: the N-th largest of 32 (128) groups' maxima of the lists' first entries is a bound, and every list is read
+// as far as it reaches that (1 x 12 x 262208 fp32, 24 candidates: 12384 entries, of which some 50 do; 64 us without, 20 us
+// with it).  Otherwise, or when more reach it than there is room for: up to 1024 entries at a time, joined with the best N of
+// the ones before, shrink to what reaches their bound (again and again while they are many) and are counted against each
+// other.
 __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamParams p) {
   __shared__ double lse[kBeamMaxK], base[kBeamMaxK];
   __shared__ int kind[kBeamMaxK];  // 0: no candidates, 1: its lists, 2: finished (one candidate)
@@ -489,11 +494,67 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamPara
     }
   }
   int cur = 0, have = 0;  // the list in use; the best candidates so far, at its front
-#pragma unroll 1
-  for (int first = 0; first < items; first += kBeamItems) {
-    if (tid == 0) sh_count[cur] = have;
+  // the N-th largest of the maxima of 32 (or 128) groups of the threads' m, for everybody
+  auto bound = [&](float m) {
+    gmax[tid] = m;
     __syncthreads();
-    const int last = min(items, first + kBeamItems);
+    if (p.N <= 32) {
+#pragma unroll
+      for (int w = 0; w < kBeamThreads / 32; ++w) m = fmaxf(m, gmax[w * 32 + lane]);
+      return warp_nth(m, p.N);
+    }
+    float4 v4;
+    v4.x = fmaxf(gmax[lane], gmax[lane + 128]);
+    v4.y = fmaxf(gmax[lane + 32], gmax[lane + 160]);
+    v4.z = fmaxf(gmax[lane + 64], gmax[lane + 192]);
+    v4.w = fmaxf(gmax[lane + 96], gmax[lane + 224]);
+    return warp_nth4(v4, p.N);
+  };
+  bool collected = false;
+  const int lists = p.K * p.splits;
+  if (items > kBeamItems && lists >= 2 * p.N) {  // of fewer lists the first entries hardly bound anything
+    if (tid == 0) sh_count[0] = 0;
+    __syncthreads();
+    // entry j of list l: its total, and where it comes from; false: there is none
+    auto entry = [&](int l, int j, double& t, unsigned int& a) {
+      const int k = l / p.splits;
+      if (kind[k] == 1) {
+        const unsigned long long key = __ldcg(keys + (size_t)l * p.N + j);
+        if (key == 0ull) return false;
+        float v;
+        int idx;
+        cand_key_decode(key, v, idx);
+        t = base[k] + ((double)v - lse[k]);
+        a = (unsigned int)k * (unsigned int)p.V + (unsigned int)idx;
+        return true;
+      }
+      t = base[k];
+      a = (unsigned int)k * (unsigned int)p.V + (unsigned int)p.pad_token;
+      return kind[k] == 2 && l == k * p.splits && j == 0;
+    };
+    float m = -INFINITY;
+    double t;
+    unsigned int a;
+    for (int l = tid; l < lists; l += kBeamThreads)
+      if (entry(l, 0, t, a)) m = fmaxf(m, __double2float_rd(t));
+    const float pivot = bound(m);
+    for (int l = tid; l < lists; l += kBeamThreads)
+      for (int j = 0; j < p.N; ++j) {
+        if (!entry(l, j, t, a) || !(__double2float_rd(t) >= pivot)) break;
+        const int pos = atomicAdd(&sh_count[0], 1);
+        if (pos >= kBeamMergeCap) break;
+        list_t[0][pos] = t;
+        list_a[0][pos] = a;
+      }
+    __syncthreads();
+    collected = sh_count[0] <= kBeamMergeCap;
+    __syncthreads();  // the count is set anew below
+  }
+#pragma unroll 1
+  for (int first = collected ? items - 1 : 0; first < items; first += kBeamItems) {
+    if (!collected && tid == 0) sh_count[cur] = have;
+    __syncthreads();
+    const int last = collected ? first : min(items, first + kBeamItems);  // collected: nothing more to read
 #pragma unroll 1
     for (int j = 0, i = first + tid; i < last; ++j, i += kBeamThreads) {
       const int k = i / per_row;
@@ -526,22 +587,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamPara
       float m = -INFINITY;
 #pragma unroll 1
       for (int i = tid; i < n; i += kBeamThreads) m = fmaxf(m, __double2float_rd(list_t[cur][i]));
-      gmax[tid] = m;
       if (tid == 0) sh_count[cur ^ 1] = 0;
-      __syncthreads();
-      float pivot;
-      if (p.N <= 32) {
-#pragma unroll
-        for (int w = 0; w < kBeamThreads / 32; ++w) m = fmaxf(m, gmax[w * 32 + lane]);
-        pivot = warp_nth(m, p.N);
-      } else {
-        float4 v4;
-        v4.x = fmaxf(gmax[lane], gmax[lane + 128]);
-        v4.y = fmaxf(gmax[lane + 32], gmax[lane + 160]);
-        v4.z = fmaxf(gmax[lane + 64], gmax[lane + 192]);
-        v4.w = fmaxf(gmax[lane + 96], gmax[lane + 224]);
-        pivot = warp_nth4(v4, p.N);
-      }
+      const float pivot = bound(m);
 #pragma unroll 1
       for (int i = tid; i < n; i += kBeamThreads) {
         const double t = list_t[cur][i];
@@ -560,7 +607,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamPara
       n = sh_count[cur];
     }
     // ranks; those that make it go out, or to the front of the other list
-    const bool end = last == items;
+    const bool end = collected || last == items;
 #pragma unroll 1
     for (int i = tid; i < n; i += kBeamThreads) {
       const double t = list_t[cur][i];

@@ -536,3 +536,38 @@ def test_first_calls_of_a_process_inside_a_capture(fs):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", _CAPTURED_FIRST], cwd=root, capture_output=True, text=True, timeout=240)
     assert done.returncode == 0 and "captured first" in done.stdout, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("kind", ["spread", "equal", "one beam", "dead", "falling"])
+@pytest.mark.parametrize("K,V,N,dtype", [(10, 50000, 20, torch.float32), (12, 70001, 24, torch.bfloat16), (5, 120000, 64, torch.float16)])
+def test_many_lists_to_join(fs, K, V, N, dtype, kind):
+    """More entries than the join holds at a time: as a rule few of them matter; with equal logits all do."""
+    R = 2
+    logits, scores = _inputs(R, K, V, dtype, seed=K + N)
+    finished = torch.zeros(R, K, dtype=torch.bool, device=_dev())
+    if kind == "equal":
+        logits = torch.ones_like(logits)
+        scores = torch.zeros_like(scores)
+    elif kind == "one beam":  # the others finished or without a score
+        finished[:, 1:3] = True
+        scores[:, 3:] = -math.inf
+    elif kind == "dead":
+        logits[0, 1:] = -math.inf
+        logits[0, 0, N // 2:] = -math.inf  # fewer candidates than asked for
+        finished[1, 0] = True
+    elif kind == "falling":  # all of the best in the first lists
+        logits = logits.sort(dim=-1, descending=True).values
+    step = fs.beam_search_step(logits, scores, num_candidates=N, finished=finished, pad_token=3)
+    ref = _reference(logits, scores, N, finished, 3)
+    if kind == "equal":  # totals of different beams are equal: the lowest beam's first tokens
+        assert step.parents.eq(0).all() and torch.equal(step.tokens.cpu(), torch.arange(N).repeat(R, 1))
+    else:
+        _check(step, ref)
+
+
+@pytest.mark.parametrize("V", [600, 1000, 1500, 2047])
+@pytest.mark.parametrize("N", [5, 24, 64])
+def test_short_rows(fs, V, N):
+    """Rows whose vectors do not fill the groups that a bound is taken from."""
+    logits, scores = _inputs(3, 4, V, torch.bfloat16, seed=V + N)
+    _check(fs.beam_search_step(logits, scores, num_candidates=N), _reference(logits, scores, N))

@@ -3,7 +3,7 @@
 // equal totals in the order of (k, v).
 //
 // Two kernels.  beam_part_kernel reads the logits once: a CTA streams a slice of one row through a ring of asynchronous
-// copies (each thread reads back only what it copied itself, so the loop has no barrier) and keeps the slice's maximum, its
+// copies (each warp, for aligned rows each thread, reads back only what it copied itself, so the loop has no barrier) and keeps the slice's maximum, its
 // sum of exponentials and its N largest logits - within a row the order of the totals is the order of the logits.
 // beam_merge_kernel, one CTA per request, joins the slices' sums and picks the N best of what they kept.
 //
@@ -157,10 +157,26 @@ __device__ __forceinline__ void copy_vector(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
+// The 16 bytes that begin `offset` bytes (below 16, a multiple of T's size) behind a 16-byte boundary in shared memory.
 template <typename T>
+__device__ __forceinline__ uint4 load_between(const uint4* at, int offset) {
+  const uint2* w = reinterpret_cast<const uint2*>(at) + (offset >> 3);
+  const uint2 a = w[0], b = w[1], c = w[2];
+  const bool odd = offset & 4;
+  const uint4 u = make_uint4(odd ? a.y : a.x, odd ? b.x : a.y, odd ? b.y : b.x, odd ? c.x : b.y);
+  if constexpr (sizeof(T) == 4) return u;
+  const uint32_t next = odd ? c.y : c.x;
+  const int bits = (offset & 2) * 8;
+  return make_uint4(__funnelshift_r(u.x, u.y, bits), __funnelshift_r(u.y, u.z, bits), __funnelshift_r(u.z, u.w, bits),
+                    __funnelshift_r(u.w, next, bits));
+}
+
+// EVEN: every row begins on a 16-byte boundary.
+template <typename T, bool EVEN>
 __global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamParams p) {
   constexpr int VE = 16 / sizeof(T);
-  __shared__ __align__(16) uint4 ring[kBeamRing][2][kBeamThreads];
+  constexpr int kWarpVecs = EVEN ? 32 : 33;  // copies of a warp for its 32 vectors
+  __shared__ __align__(16) uint4 ring[kBeamRing][2][kBeamThreads / 32 * kWarpVecs];
   __shared__ __align__(16) float gmax[128];
   __shared__ float sh_pivot;
   __shared__ int sh_vecs, sh_count;
@@ -174,36 +190,55 @@ __global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamPa
   const int row = blockIdx.y, split = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if ((p.finished && p.finished[row]) || !beam_live(p, row)) return;  // the merge does not look at such rows either
   const T* x = reinterpret_cast<const T*>(p.logits) + (row / p.K) * p.stride_r + (row % p.K) * p.stride_k;
-  // whole vectors on 16-byte boundaries, behind up to VE - 1 elements before the first boundary and before as many at the
-  // end: the first and the last slice's single elements
-  const int lead = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T), p.V);
-  const int vecs = (p.V - lead) / VE, tail = lead + vecs * VE;
+  // A row is cut into vectors from its first element on, wherever it lies, so that rows with the same values have the
+  // same sums to the last bit: equal totals of two beams are told apart by (beam, token) alone.  Copies are the 16 bytes on
+  // boundaries.  Where a row begins `shift` elements behind one, vector v is the end of copy v and the beginning of copy v + 1,
+  // the next lane's, and two lanes of a warp fetch what follows its last vectors.  (64 x 8 x 128257 bf16, 16 candidates: 58 us
+  // instead of the 50 us of 128256.)  The last VE to 2 VE - 1 elements, so that no copy ends behind the row, are the last
+  // slice's singles.
+  const int shift = EVEN ? 0 : (int)(reinterpret_cast<uintptr_t>(x) & 15) / (int)sizeof(T);
+  const int vecs = max(p.V / VE - 1, 0), tail = vecs * VE;
   const int v_begin = min(split * p.iters * kBeamThreads, vecs), v_end = min(v_begin + p.iters * kBeamThreads, vecs);
-  const int singles = (split == 0 ? lead : 0) + (split == p.splits - 1 ? p.V - tail : 0);
-  const T* xv = x + lead;
+  const int singles = split == p.splits - 1 ? p.V - tail : 0;
+  const int copy_end = !EVEN && v_end > v_begin ? v_end + 1 : v_end, place = warp * kWarpVecs + lane;
+  const T* boundary = x - shift;
 
   auto fetch = [&](int v, int slot) {  // vectors v and v + 256 of the row, for this thread
-    if (v < v_end) copy_vector(&ring[slot][0][tid], xv + (size_t)v * VE);
-    if (v + kBeamThreads < v_end) copy_vector(&ring[slot][1][tid], xv + (size_t)(v + kBeamThreads) * VE);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      // (copy 0 begins before the row unless that begins on a boundary)
+      if (v + h * kBeamThreads < copy_end && (EVEN || h > 0 || v > 0 || shift == 0))
+        copy_vector(&ring[slot][h][place], boundary + (size_t)(v + h * kBeamThreads) * VE);
+    if constexpr (!EVEN) {
+      const int h = 31 - lane, next = v + h * (kBeamThreads + 1);  // lane 31: its own vector's sequel; lane 30: lane 31's other one's
+      if (h < 2 && next < v_end) copy_vector(&ring[slot][h][warp * kWarpVecs + 32], boundary + (size_t)(next + 1) * VE);
+    }
     asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (!EVEN && shift && v_begin == 0 && v_end > 0 && tid < VE - shift) reinterpret_cast<T*>(ring[0][0])[shift + tid] = x[tid];
+  auto take = [&](int slot, int h) {  // this thread's vector, once the warp's copies are there
+    if constexpr (EVEN)
+      return ring[slot][h][place];
+    else
+      return load_between<T>(&ring[slot][h][place], shift * (int)sizeof(T));
   };
 #pragma unroll
   for (int i = 0; i < kBeamRing - 1; ++i) fetch(v_begin + 2 * i * kBeamThreads + tid, i);
   float single = -INFINITY;
   int single_at = 0;
-  if (tid < singles) {  // at most 2 (VE - 1) threads
-    const int head = split == 0 ? lead : 0;
-    single_at = tid < head ? tid : tail + tid - head;
+  if (tid < singles) {  // at most 2 VE - 1 threads
+    single_at = tail + tid;
     single = fmaxf((float)x[single_at], -INFINITY);
   }
   if (tid == 0) sh_vecs = sh_count = 0;
 
   // bound and first reference of the exponentials from the first vectors (fmaxf drops NaN)
   asm volatile("cp.async.wait_group %0;" ::"n"(kBeamRing - 1 - kBeamFirst / 2) : "memory");
+  if constexpr (!EVEN) __syncwarp();
   float m = single;
 #pragma unroll
   for (int i = 0; i < kBeamFirst; ++i)
-    if (v_begin + i * kBeamThreads + tid < v_end) m = fmaxf(m, beam_vec_max<T>(ring[i / 2][i % 2][tid]));
+    if (v_begin + i * kBeamThreads + tid < v_end) m = fmaxf(m, beam_vec_max<T>(take(i / 2, i % 2)));
   // The N-th largest of 32 groups' maxima (8 lanes each; up to 32 candidates), or of 128 (2 lanes): into sh_pivot; the
   // largest: returned.
   // Few vectors leave groups of 8 lanes empty, and the bound would be -inf (64 x 12 x 1500 bf16, 24
@@ -281,10 +316,12 @@ __global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamPa
 #pragma unroll 1
   for (int i = 0, v = v_begin + tid; i < p.iters / 2; ++i, v += 2 * kBeamThreads) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kBeamRing - 2) : "memory");
+    // other lanes' copies are there; and every lane has read the slot before this one, which is filled next
+    if constexpr (!EVEN) __syncwarp();
     const int slot = i % kBeamRing;
     uint4 u0 = make_uint4(kNone, kNone, kNone, kNone), u1 = u0;
-    if (v < v_end) u0 = ring[slot][0][tid];
-    if (v + kBeamThreads < v_end) u1 = ring[slot][1][tid];
+    if (v < v_end) u0 = take(slot, 0);
+    if (v + kBeamThreads < v_end) u1 = take(slot, 1);
     fetch(v + 2 * (kBeamRing - 1) * kBeamThreads, (i + kBeamRing - 1) % kBeamRing);
     const float vm0 = beam_vec_max<T>(u0), vm1 = beam_vec_max<T>(u1), vm = fmaxf(vm0, vm1);
     m = fmaxf(m, vm);
@@ -332,12 +369,12 @@ __global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamPa
   if (vecs_noted <= kBeamVecCap) {
 #pragma unroll 1
     for (int i = tid; i < vecs_noted * VE; i += kBeamThreads)
-      offer((float)reinterpret_cast<const T*>(vec_data)[i], lead + vec_list[i / VE] * VE + i % VE);
+      offer((float)reinterpret_cast<const T*>(vec_data)[i], vec_list[i / VE] * VE + i % VE);
     if (tid < singles) offer(single, single_at);
   }
   __syncthreads();
   int n = sh_count;
-  const int from = split == 0 ? 0 : lead + v_begin * VE, to = split == p.splits - 1 ? p.V : lead + v_end * VE;
+  const int from = v_begin * VE, to = split == p.splits - 1 ? p.V : v_end * VE;
   const size_t part = (size_t)row * p.splits + split;
   unsigned long long* out = p.keys + part * p.N;
   if (tid == kBeamThreads - 1) {  // the last warp: the first ones rank the list

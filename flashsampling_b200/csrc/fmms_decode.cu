@@ -206,6 +206,15 @@ static size_t beam_workspace(int R, int K, int V, int N, int dtype) {
   return parts * N * 8 + parts * 8 + parts * 4;
 }
 
+template <typename T>
+static void beam_launch_part(const BeamParams& p, dim3 grid, cudaStream_t stream) {
+  const long long between = (p.R > 1 ? p.stride_r : 0) | (p.K > 1 ? p.stride_k : 0);  // a set low bit: so has one of the strides
+  if (reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && between % (16 / (int)sizeof(T)) == 0)
+    beam_part_kernel<T, true><<<grid, kBeamThreads, 0, stream>>>(p);
+  else
+    beam_part_kernel<T, false><<<grid, kBeamThreads, 0, stream>>>(p);
+}
+
 int reorder_beams_rounded(int K) { return K <= 2 ? 2 : K <= 4 ? 4 : K <= 8 ? 8 : K <= 16 ? 16 : K <= 32 ? 32 : 64; }
 
 // Bytes of a column: what divides the state's address and strides.
@@ -381,11 +390,11 @@ int fmms_beam_step(const void* logits, int dtype, long long stride_r, long long 
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const dim3 grid((unsigned)p.splits, (unsigned)(R * K));
   if (dtype == FMMS_BF16)
-    beam_part_kernel<__nv_bfloat16><<<grid, kBeamThreads, 0, s>>>(p);
+    beam_launch_part<__nv_bfloat16>(p, grid, s);
   else if (dtype == FMMS_F16)
-    beam_part_kernel<__half><<<grid, kBeamThreads, 0, s>>>(p);
+    beam_launch_part<__half>(p, grid, s);
   else
-    beam_part_kernel<float><<<grid, kBeamThreads, 0, s>>>(p);
+    beam_launch_part<float>(p, grid, s);
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   return launch_behind(beam_merge_kernel, dim3((unsigned)R), kBeamThreads, 0, s, p);
 }

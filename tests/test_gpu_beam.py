@@ -571,3 +571,24 @@ def test_short_rows(fs, V, N):
     """Rows whose vectors do not fill the groups that a bound is taken from."""
     logits, scores = _inputs(3, 4, V, torch.bfloat16, seed=V + N)
     _check(fs.beam_search_step(logits, scores, num_candidates=N), _reference(logits, scores, N))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [7, 1501, 32003, 50257, 128257])
+def test_equal_beams_that_lie_anywhere(fs, V, dtype):
+    """Beams with the same logits and scores, each in a row of its own: an odd number of tokens puts every row elsewhere
+    between two 16-byte boundaries, and equal totals come in the order of (beam, token) all the same."""
+    R, K, N = 2, 8, 24
+    row = _inputs(R, 1, V, dtype, seed=V)[0]
+    wide = torch.full((R, K, V + 6), math.nan, dtype=dtype, device=_dev())  # NaN around the rows: no row reads beyond itself
+    even = torch.zeros((R, K, V + 8 - V % 8), dtype=dtype, device=_dev())
+    even[..., :V] = row
+    for logits in (row.expand(R, K, V).contiguous(), even[..., :V], wide[..., 1:V + 1], wide[..., 4:V + 4]):
+        logits.copy_(row.expand(R, K, V))
+        step = fs.beam_search_step(logits, torch.full((R, K), -3.7, device=_dev()), num_candidates=N)
+        for r in range(R):
+            x = row[r, 0].tolist()
+            top = sorted(range(V), key=lambda v: (-x[v], v))[:N]
+            want = sorted(((k, v) for k in range(K) for v in top), key=lambda c: (-x[c[1]], c[0], c[1]))[:N]
+            assert list(zip(step.parents[r].tolist(), step.tokens[r].tolist())) == want
+        wide.fill_(math.nan)

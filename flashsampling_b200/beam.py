@@ -46,7 +46,10 @@ def beam_search_step(
     finished beam goes on as it is: its one candidate is ``pad_token`` with its unchanged score.  Where fewer than
     ``num_candidates`` exist, the rest is score ``-inf``, token ``-1``, parent ``min(position, beams - 1)``.
 
-    Log-softmax and totals are formed in 64 bits.  Up to 64 beams and 64 candidates.  Rows may lie anywhere
+    Exponentials and the sums of a thread are fp32, joined sums, logarithms and totals 64-bit: a log-softmax is within
+    ``(15 + ln vocab) 2^-24`` (2e-6 for 2^18 tokens; measured 1e-7).  Candidates of two beams that lie closer together may
+    come in either order, which may also change with the size of the batch; within a beam, and between beams of equal logits and
+    scores, the order is exact.  Up to 64 beams and 64 candidates.  Rows may lie anywhere
     (``logits[..., :vocab]`` of a padded head needs no copy), their elements must be consecutive.  No gradients."""
     if not (logits.is_cuda and scores.is_cuda):
         raise RuntimeError("beam_search_step requires CUDA tensors (there is no CPU path)")

@@ -397,7 +397,10 @@ int fmms_query_int4_workspace(int V, int D, int group, int B, size_t* bytes);
 /*
  * One step of a beam search.  For each of R requests with K beams: of all continuations (beam k, token v) the N with
  * the largest scores[r, k] + logits[r, k, v] - ln sum_v exp(logits[r, k, v]), in descending order, equal ones in the
- * order of (k, v).  Sums and totals are formed in 64 bits.
+ * order of (k, v).  Exponentials and the sums of a thread are fp32, joined sums, logarithms and totals 64-bit: a total
+ * is within (15 + ln V) 2^-24 plus the rounding of the output (2e-6 for 2^18 tokens; measured 1e-7).  Candidates of
+ * two beams that lie closer together may come in either order, which may also change with R * K; within a beam, and between
+ * beams of equal logits and scores, the order is exact.
  *
  *   logits       row (r, k) starts at r * stride_r + k * stride_k elements; V consecutive bf16, fp16 or fp32 values.
  *                NaN and -inf are tokens that may not follow.  A row with +inf, or with nothing above -inf, gives no

@@ -592,3 +592,64 @@ def test_equal_beams_that_lie_anywhere(fs, V, dtype):
             want = sorted(((k, v) for k in range(K) for v in top), key=lambda c: (-x[c[1]], c[0], c[1]))[:N]
             assert list(zip(step.parents[r].tolist(), step.tokens[r].tolist())) == want
         wide.fill_(math.nan)
+
+
+def _lse_errors(fs, logits):
+    """Errors of the log-sum-exps of rows [K, V]: a score that cancels the best token's log-probability leaves a total so
+    near zero that the fp32 output shows them."""
+    x = logits.cpu().double()
+    lse, top = torch.logsumexp(x, 1), x.amax(1)
+    scores = (lse - top).float()
+    step = [fs.beam_search_step(logits[k].view(1, 1, -1), scores[k].view(1, 1).to(_dev()), num_candidates=1).scores for k in range(len(x))]
+    return torch.cat(step).view(-1).cpu().double() - (scores.double() + (top - lse))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [40, 5000, 262208])
+def test_log_sum_exp_within_what_is_claimed(fs, V, dtype):
+    """Per exponential 2^-22 for the special-function unit and 2^-24 |x - max| for the rounding of the difference, whose
+    mean over the softmax is at most ln V; 11 fp32 additions of 2^-24 (3 in a pass over two vectors, 8 passes); the rest
+    is fp64: (4 + 11 + ln V) 2^-24 relative, which is the logarithm's absolute error (below 2e-6 for 2^18 tokens)."""
+    g = torch.Generator().manual_seed(V)
+    rows = [
+        torch.randn(V, generator=g) * 2.2,  # a wide one
+        torch.randn(V, generator=g) * 8,  # a peaked one
+        torch.rand(V, generator=g) * 0.7,  # a flat one
+        torch.where(torch.rand(V, generator=g) < 0.5, -0.3, 0.0),  # two values
+        torch.randn(V, generator=g) * 2.2 - 30,  # log-probabilities
+        torch.cat([torch.tensor([11.3, 11.1, 10.7]), torch.randn(V - 3, generator=g)]),  # three tokens with the mass
+        torch.linspace(-20, 20, V),
+    ]
+    errors = _lse_errors(fs, torch.stack(rows).to(dtype).to(_dev()))
+    assert bool((errors.abs() <= (15 + math.log(V)) * 2.0**-24).all()), errors
+
+
+def test_exponentials_carry_the_rounding_of_their_arguments(fs):
+    """Tokens d below the maximum, where d log2(e) rounds by half a step of fp32: 2^-20, with what fp32 cuts off log2(e)
+    8e-7 of their share of the sum.  Carried along, what is left is the special-function unit's 2^-22: d is a bf16
+    number, a thread's sum of 8 or 16 equal numbers in pairs is exact, and the maxima (one in 4096 tokens: every slice's
+    reference) stand alone in their threads, whose other tokens (within 8 of a multiple of 1024) are masked."""
+    V, log2e = 262208, 1.4426950408889634
+    d = -torch.arange(11.125, 12, 0.0625)
+    off = d.double() * log2e - (d * torch.tensor(log2e, dtype=torch.float32)).double()
+    at = int(off.abs().argmax())
+    x = torch.full((1, V), float(d[at]))
+    x[:, torch.arange(V) % 1024 < 8] = -math.inf
+    x[:, ::4096] = 0
+    mass = int((x == d[at]).sum()) * math.exp(float(d[at]))
+    share = mass / (mass + int((x == 0).sum()))
+    tol = share * 2.0**-22 + 1e-9
+    assert share * (float(off[at].abs()) * math.log(2) - 2.0**-22) > 2 * tol  # without it, errors are larger than this
+    for dtype in (torch.bfloat16, torch.float32):
+        assert abs(float(_lse_errors(fs, x.to(dtype).to(_dev()))[0])) <= tol
+
+
+def test_sums_join_in_more_than_32_bits(fs):
+    """Equal logits: exponentials and a thread's sums are exact, and 2^24 + 3 of them are more than fp32 can count.  A beam
+    with one token fewer has probabilities that are larger by 6e-8, and comes first."""
+    V, K = (1 << 24) + 3, 2
+    logits = torch.zeros(K, V, dtype=torch.bfloat16, device=_dev())
+    logits[1, 7] = -math.inf
+    assert bool((_lse_errors(fs, logits).abs() <= 1e-10).all())
+    step = fs.beam_search_step(logits[None], torch.full((1, K), -2.5, device=_dev()), num_candidates=5)
+    assert step.parents[0].tolist() == [1] * 5 and step.tokens[0].tolist() == [0, 1, 2, 3, 4]

@@ -15,6 +15,7 @@ from typing import NamedTuple, Sequence
 import torch
 
 from . import _lib
+from .core import _status_word
 from .int4 import Int4Weight, int4_linear
 
 __all__ = ["BeamStep", "beam_search_step", "reorder_beams", "BeamSearch"]
@@ -266,6 +267,7 @@ class BeamSearch:
             raise RuntimeError("BeamSearch requires a head on a GPU (there is no CPU path)")
         if requests < 1 or max_steps < 1 or not 1 <= beams <= 64:
             raise ValueError("BeamSearch takes at least one request and one step, and 1 to 64 beams")
+        _status_word(dev)  # here, for the first step may be inside a capture
         self.requests, self.beams, self.max_steps = requests, beams, max_steps
         self.eos_token, self.pad_token = eos_token, pad_token
         self.tokens = torch.full((requests * beams, max_steps), pad_token, dtype=torch.int64, device=dev)

@@ -80,10 +80,20 @@ def _fp8_staging(device: torch.device, stream_id: int, d: int, b: int, s: int) -
     return st
 
 
-def _status_word(device: torch.device) -> torch.Tensor:
+def _status_word(device: torch.device) -> torch.Tensor | None:
+    """The device's status word, made at the first use outside of a capture; ``None`` if it is missing during one.
+
+    A word made in a capture would lie in that graph's memory, unwritten until the first replay and cleared by every
+    one.  It is zero before anybody sees it, whatever stream that is on."""
     st = _status.get(device.index)
     if st is None:
-        st = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                return None
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                st = torch.zeros(1, dtype=torch.int32, device=device)
+            stream.synchronize()
         _status[device.index] = st
     return st
 
@@ -92,7 +102,8 @@ def check_status(device: torch.device | None = None) -> None:
     """Synchronise and raise if a kernel recorded a device-side time-out.
 
     The sampling call itself never synchronises; call this where a sync is
-    acceptable (tests, benchmarks, shutdown).
+    acceptable (tests, benchmarks, shutdown).  A graph whose capture held the
+    process's first call on a device has no word to record to.
     """
     devs = [device.index] if device is not None else list(_status)
     for idx in devs:
@@ -270,7 +281,7 @@ def fused_mm_sample(
         seed_arg, v_begin, flags, noise_ptr, noise_ld,
         logits.data_ptr() if logits is not None else None, out.data_ptr(),
         vals.data_ptr() if vals is not None else None, ws.data_ptr(), ws.numel(),
-        status.data_ptr(), stream.cuda_stream,
+        status.data_ptr() if status is not None else None, stream.cuda_stream,
     )
     fused_tp = tp.size > 1 and getattr(exchange, "fused", False) and B * num_samples <= exchange.max_items \
         and not two_stage and B <= 256  # larger batches run as several launches, then one exchange
@@ -491,7 +502,7 @@ class PreparedSampler:
         ws = _workspace(self.dev, stream, nbytes)
         status = _status_word(self.dev)
         c.workspace, c.workspace_bytes = ws.data_ptr(), ws.numel()
-        c.status_dev = status.data_ptr()
+        c.status_dev = status.data_ptr() if status is not None else None
         c.stream = stream
         keep += [ws, status, self.weights]
         call = _PreparedCall(c, tuple(keep))

@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from .core import _status_word
 from .quant import int4_group_ok, quantize_groups_int4
 
 __all__ = ["Int4Weight", "int4_linear"]
@@ -59,6 +60,8 @@ class Int4Weight:
         )
         for name, value in zip(self.__slots__, (qweight, scales, zeros, rows, cols, group, args)):
             object.__setattr__(self, name, value)
+        if qweight.is_cuda:
+            _status_word(qweight.device)  # here, for the first product may be inside a capture
 
     def __setattr__(self, name, value):
         raise AttributeError("an Int4Weight keeps its tensors: make a new one")
@@ -187,8 +190,6 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
 
 
 def _launch(x, stride, weight, b, out, out_stride, index):
-    from .core import _status_word  # core is imported first
-
     qw, scales, scale_dtype, zeros, rows, cols, group = weight._args
     key = (rows, cols, group, b)
     nbytes = _ws_bytes.get(key)
@@ -196,8 +197,13 @@ def _launch(x, stride, weight, b, out, out_stride, index):
         nbytes = _ws_bytes[key] = _lib.query_int4_workspace(*key)
     # from torch's allocator on every call: calls on several streams, or in several captured graphs, share nothing
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    status = None
+    if b > 8:  # up to eight rows there are no waits between warps
+        status = _status_word(x.device)
+        if status is None:
+            raise RuntimeError("int4_linear has no status word yet, and cannot make one in a capture: make an Int4Weight on the device before it")
     return _lib.load().fmms_int4_linear(
         x.data_ptr(), _DTYPES[x.dtype], stride, qw, scales, scale_dtype, zeros, rows, cols, group, b,
         out.data_ptr(), _DTYPES[out.dtype], out_stride, ws.data_ptr() if nbytes else None, nbytes,
-        _status_word(x.device).data_ptr() if b > 8 else None,  # up to eight rows: no waits between warps
+        status.data_ptr() if status is not None else None,
         torch._C._cuda_getCurrentRawStream(index))

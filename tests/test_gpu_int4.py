@@ -362,3 +362,63 @@ def test_refusals(fs):
         fs.int4_linear(x.clone().requires_grad_(), w)
     with torch.no_grad():
         fs.int4_linear(x.clone().requires_grad_(), w)
+
+
+_STATUS = """
+import torch
+import flashsampling_b200 as fs
+from flashsampling_b200 import _lib, core
+dev = torch.device("cuda", 0)
+g = torch.Generator().manual_seed(0)
+cpu = fs.Int4Weight.from_rows(torch.randint(0, 16, (300, 256), generator=g, dtype=torch.uint8), torch.full((300, 2), 0.01).bfloat16())
+x = torch.randn(20, 256, generator=g).bfloat16().to(dev)
+dense = torch.randn(512, 256, generator=g).bfloat16().to(dev)
+qweight, scales = cpu.qweight.to(dev), cpu.scales.to(dev)
+junk = [torch.full((1 << 20,), -1, dtype=torch.int32, device=dev) for _ in range(4)]
+del junk
+torch.cuda.synchronize()
+
+# a weight of a capture, before anything made the status word: no call that needs it, and no word in the graph
+early = torch.cuda.CUDAGraph()
+with torch.cuda.graph(early):
+    w = fs.Int4Weight(qweight, scales, None, 300, 256)
+    few = fs.int4_linear(x[:3], w)
+    try:
+        fs.int4_linear(x, w)
+        raise SystemExit("a product without a status word")
+    except RuntimeError as e:
+        assert "status word" in str(e)
+    ids = fs.fused_mm_sample(dense, x, 1, None, 0, greedy_sampling=True)
+assert not core._status
+fs.check_status()
+early.replay()
+torch.cuda.synchronize()
+assert torch.equal(ids[:, 0], (x.double() @ dense.double().T).argmax(1))
+
+w = cpu.to(dev)
+assert torch.equal(few, fs.int4_linear(x[:3], w))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = fs.int4_linear(x, w)
+fs.check_status()  # nothing has run yet
+core._status[0].fill_(_lib.ERR_TIMEOUT)  # as an earlier call's time-out
+graph.replay()
+try:
+    fs.check_status()
+    raise SystemExit("the replay cleared the word")
+except _lib.FmmsError:
+    pass
+fs.check_status()
+assert torch.equal(y, fs.int4_linear(x, w))
+print("status kept")
+"""
+
+
+def test_status_word_of_a_process_whose_first_calls_are_captured(fs):
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", _STATUS], cwd=root, capture_output=True, text=True, timeout=240)
+    assert done.returncode == 0 and "status kept" in done.stdout, done.stdout[-500:] + done.stderr[-2000:]

@@ -69,7 +69,8 @@ def quantize_groups_int4(
 
     Symmetric: the zero point is 8 everywhere (``zeros`` is ``None``) and the group's largest magnitude becomes +-7.
     Otherwise the group's range, widened to hold 0, is spread over the 16 codes.  ``scale_dtype`` is bf16 or fp16
-    (default: the weight's own type if it is one of them, else bf16); codes are chosen for the rounded scale."""
+    (default: the weight's own type if it is one of them, else bf16); codes are chosen for the rounded scale.  A weight that is not
+    finite, or whose scales ``scale_dtype`` cannot hold, is refused (which waits for the GPU, once)."""
     if w.ndim != 2 or not w.is_floating_point():
         raise ValueError("expected a floating-point [rows, columns] tensor")
     if not int4_group_ok(group_size, w.shape[1]):
@@ -83,6 +84,7 @@ def quantize_groups_int4(
     q = torch.empty((rows, cols), dtype=torch.uint8, device=w.device)
     scales = torch.empty((rows, groups), dtype=scale_dtype, device=w.device)
     zeros = None if symmetric else torch.empty((rows, groups), dtype=torch.uint8, device=w.device)
+    finite = torch.ones((), dtype=torch.bool, device=w.device)
     step = 8192
     for r0 in range(0, rows, step):
         blk = w[r0:r0 + step].float().view(-1, groups, group_size)
@@ -92,6 +94,7 @@ def quantize_groups_int4(
             lo, hi = blk.amin(-1).clamp_max(0), blk.amax(-1).clamp_min(0)
             s = (hi - lo) / 15
         s = s.to(scale_dtype)
+        finite &= s.isfinite().all()
         s = torch.where(s > 0, s, torch.ones_like(s))  # an all-zero group, or one whose scale rounds to zero
         z = torch.full_like(s, 8.0) if symmetric else torch.round(-lo / s.float()).clamp(0, 15).to(s.dtype)
         code = torch.round(blk / s.float()[..., None]) + z.float()[..., None]
@@ -99,4 +102,6 @@ def quantize_groups_int4(
         scales[r0:r0 + step] = s
         if zeros is not None:
             zeros[r0:r0 + step] = z.to(torch.uint8)
+    if not bool(finite):
+        raise ValueError(f"the weight holds values that are not finite, or too large for a scale in {scale_dtype}")
     return q, scales, zeros

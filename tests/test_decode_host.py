@@ -248,3 +248,21 @@ def test_a_weight_keeps_its_tensors():
             setattr(w, name, None)
     again = pickle.loads(pickle.dumps(w))
     assert again.shape == w.shape and torch.equal(again.dequantize(), w.dequantize())
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_quantiser_refuses_what_a_scale_cannot_hold(symmetric):
+    """A scale of infinity would make every weight of its group NaN."""
+    for value, dtype in ((6e5, torch.float16), (float("inf"), torch.bfloat16), (float("nan"), torch.bfloat16), (-float("inf"), torch.float16)):
+        w = torch.zeros(3, 64)
+        w[1, 40] = value
+        if not symmetric:
+            w[1, 41] = -value
+        with pytest.raises(ValueError, match="finite"):
+            quantize_groups_int4(w, 32, symmetric, dtype)
+        with pytest.raises(ValueError, match="finite"):
+            fs.Int4Weight.quantize(w, 32, symmetric, dtype)
+    w = torch.full((2, 32), 4e5)  # the largest scales of fp16 are scales
+    w[1] = -4e5
+    back = fs.Int4Weight.from_rows(*quantize_groups_int4(w, 32, symmetric, torch.float16)).dequantize()
+    assert bool(((back - w).abs() <= 4e5 * (0.5 / 7 + 2.0**-10)).all())

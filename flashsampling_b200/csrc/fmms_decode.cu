@@ -15,7 +15,7 @@
 namespace fmms {
 
 constexpr int kDecodeMaxDevices = 16;
-constexpr int kInt4SmemLimit = 230000;  // of 232448 bytes a CTA may have; the rest: static shared memory
+constexpr int kInt4SmemLimit = 230000;  // of 232448 bytes a CTA may have; the rest: static shared memory and alignment
 
 static int decode_num_sms(int* dev_out, int* sms_out) {
   static std::atomic<int> sms[kDecodeMaxDevices];
@@ -133,7 +133,7 @@ static void int4_mma_plan(Int4MmaPlan& pl, int D, int B, int group, bool zeros) 
   pl.x_stages = min(kInt4MmaMaxX, (kInt4SmemLimit - weights - scales) / int4_x_bytes(pl.n, gr));
   pl.ring_off = pl.x_stages * int4_x_bytes(pl.n, gr);
   pl.scale_off = pl.ring_off + weights;
-  pl.smem = pl.scale_off + scales;
+  pl.smem = pl.scale_off + scales + kInt4MmaAlign;
 }
 
 // staged x, then the exponents of its rows
@@ -149,7 +149,7 @@ static int int4_mma_launch(const Int4MmaParams& p, const Int4MmaPlan& pl, int de
     auto* kernel = int4_mma_kernel<NC, GR, ZP>;
     static std::atomic<bool> ready[kDecodeMaxDevices];
     if (!ready[dev].load(std::memory_order_acquire)) {
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kInt4SmemLimit) != cudaSuccess) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kInt4SmemLimit + kInt4MmaAlign) != cudaSuccess) {
         cudaGetLastError();
         return kErrCuda;
       }

@@ -117,7 +117,7 @@ __device__ __forceinline__ void int4_store(const Int4Params& p, int b, int v, fl
 // GR: columns of a group, at most 128; ZP: zero points given.
 template <int GR, bool ZP>
 __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_linear_kernel(const Int4Params p) {
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem_parts[];
   constexpr int kChunks = kInt4Unit / kInt4Chunk, kGroups = int4_unit_groups(GR);  // of a unit
   constexpr int kStage = int4_stage_bytes(GR), S = kInt4Stages;
   constexpr int kScaleOff = 2 * kChunks * 512, kZeroOff = kScaleOff + 2 * kGroups * 32;
@@ -130,11 +130,11 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_linear_kernel(const I
   const int g = lane >> 2, t = lane & 3;
   const int nb = p.B;
 
-  uint4* xfrag = reinterpret_cast<uint4*>(smem);
-  float* xs = reinterpret_cast<float*>(smem + p.xs_off);      // [groups of a phase][kInt4Rows]
-  float* xs32 = reinterpret_cast<float*>(smem + p.xs32_off);  // the same for 32 columns each (groups of 32: xs)
-  float* pieces = reinterpret_cast<float*>(smem + p.piece_off);  // [warps][8][32]
-  const uint8_t* ring = smem + p.ring_off + warp * (S * kStage);
+  uint4* xfrag = reinterpret_cast<uint4*>(smem_parts);
+  float* xs = reinterpret_cast<float*>(smem_parts + p.xs_off);      // [groups of a phase][kInt4Rows]
+  float* xs32 = reinterpret_cast<float*>(smem_parts + p.xs32_off);  // the same for 32 columns each (groups of 32: xs)
+  float* pieces = reinterpret_cast<float*>(smem_parts + p.piece_off);  // [warps][8][32]
+  const uint8_t* ring = smem_parts + p.ring_off + warp * (S * kStage);
   const uint32_t ring_at = smem_u32(ring);
 
   // x: a thread has one row and one t, and 8 of every 32 columns: the 16 bytes of one lane's operands.  The first loads go

@@ -39,6 +39,7 @@ constexpr int kInt4MmaPass = 64;       // rows of x in a pass, at most
 constexpr int kInt4MmaRing = 4;        // steps in a warp's ring (every second one is its own)
 constexpr int kInt4MmaMaxX = 6;        // steps of x in shared memory
 constexpr int kInt4MmaScaleRing = 8;   // steps of scales
+constexpr int kInt4MmaAlign = 1024;    // of the shared memory of a CTA, whose dynamic part has as many bytes more
 // A step is what changes hands at a time: 256 columns, for barriers, not arithmetic, set the pace of a shorter one; 128 where
 // tensor memory (of a slot: operands at 64 columns a unit, zero points 8, accumulators at a column per row of x and group)
 // does not hold two of them.
@@ -223,7 +224,9 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // NC: rows of x in a pass (16, 32, 48 or 64).
 template <int NC, int GR, bool ZP>
 __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4MmaParams p) {
-  extern __shared__ __align__(1024) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  // swizzled operands begin on 1 KiB boundaries
+  uint8_t* const smem = smem_raw + ((kInt4MmaAlign - (smem_u32(smem_raw) & (kInt4MmaAlign - 1))) & (kInt4MmaAlign - 1));
   constexpr int kGroups = int4_unit_groups(GR), kSteps = GR / 16;
   constexpr int kStepU = int4_step_units(GR, NC), kStepG = int4_step_groups(GR, NC);
   constexpr int kXBytes = int4_x_bytes(NC, GR);

@@ -266,3 +266,23 @@ def test_quantiser_refuses_what_a_scale_cannot_hold(symmetric):
     w[1] = -4e5
     back = fs.Int4Weight.from_rows(*quantize_groups_int4(w, 32, symmetric, torch.float16)).dequantize()
     assert bool(((back - w).abs() <= 4e5 * (0.5 / 7 + 2.0**-10)).all())
+
+
+def test_dynamic_shared_memory_has_one_alignment_per_name():
+    """Kernels of a translation unit that declare the same array with different alignments get one of them."""
+    import re
+
+    from flashsampling_b200 import build
+
+    def unit(path, seen):
+        if path in seen or not path.exists():
+            return ""
+        seen.add(path)
+        text = path.read_text()
+        return text + "".join(unit((path.parent / name).resolve(), seen) for name in re.findall(r'#include "([^"]+)"', text))
+
+    for source in build.SOURCES:
+        found = {}
+        for align, name in re.findall(r"extern __shared__ (?:__align__\((\d+)\) )?[\w ]+? (\w+)\[\]", unit(source.resolve(), set())):
+            found.setdefault(name, set()).add(align)
+        assert found and all(len(aligns) == 1 for aligns in found.values()), (source.name, found)

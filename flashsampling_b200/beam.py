@@ -15,7 +15,7 @@ from typing import NamedTuple, Sequence
 import torch
 
 from . import _lib
-from .core import _status_word
+from .core import _refuse_gradients, _status_word
 from .int4 import Int4Weight, int4_linear
 
 __all__ = ["BeamStep", "beam_search_step", "reorder_beams", "BeamSearch"]
@@ -85,8 +85,7 @@ def beam_search_step(
         raise ValueError(f"pad_token must be one of the {V} tokens")
     if V > 1 and logits.stride(-1) != 1:
         raise ValueError("the logits of a row must be consecutive")
-    if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
-        raise RuntimeError("beam_search_step has no backward pass: call it under torch.no_grad()")
+    _refuse_gradients("beam_search_step", logits, scores)
     if not scores.is_contiguous():
         scores = scores.contiguous()
     done = None
@@ -214,8 +213,7 @@ def reorder_beams(
     for s in states:
         if s.device != dev:
             raise ValueError(f"a state is on {s.device}, parents on {dev}")
-        if s.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("reorder_beams works in place and has no backward pass: call it under torch.no_grad()")
+        _refuse_gradients("reorder_beams (in place)", s)
         if s.is_complex() or s.is_sparse or s.is_quantized:
             raise TypeError("states must be plain dense tensors")
         d = dim + s.ndim if dim < 0 else dim

@@ -18,6 +18,7 @@ from dataclasses import dataclass
 from typing import Callable, Protocol
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .tp_info import TP1, TPInfo
@@ -96,6 +97,14 @@ def _status_word(device: torch.device) -> torch.Tensor | None:
             stream.synchronize()
         _status[device.index] = st
     return st
+
+
+def _refuse_gradients(where: str, *tensors: torch.Tensor) -> None:
+    """Raise where autograd would want to go through one of ``tensors``, backward or forward."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{where} has no backward pass: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{where} has no forward-mode derivative, and a tensor carries a tangent")
 
 
 def check_status(device: torch.device | None = None) -> None:

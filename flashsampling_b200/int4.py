@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .core import _status_word
+from .core import _refuse_gradients, _status_word
 from .quant import int4_group_ok, quantize_groups_int4
 
 __all__ = ["Int4Weight", "int4_linear"]
@@ -151,8 +151,7 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
     dev = weight.qweight.device
     if x.device != dev:
         raise ValueError(f"x is on {x.device}, the weight on {dev}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("int4_linear has no backward pass: call it under torch.no_grad()")
+    _refuse_gradients("int4_linear", x)
     x2 = x if x.ndim == 2 else x.reshape(-1, weight.cols)
     if x2.stride(1) != 1 or x2.stride(0) < weight.cols:
         x2 = x2.contiguous()
@@ -175,6 +174,7 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
             raise ValueError("out must have consecutive rows of consecutive elements")
         if out.requires_grad:
             raise RuntimeError("out must not require gradients")
+        _refuse_gradients("int4_linear", out)
     if b == 0:
         return out
     stride = x2.stride(0) if b > 1 else max(x2.stride(0), weight.cols)

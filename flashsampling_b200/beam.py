@@ -13,6 +13,7 @@ import math
 from typing import NamedTuple, Sequence
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .core import _refuse_gradients, _status_word
@@ -239,6 +240,7 @@ def reorder_beams(
             rc = _lib.load().fmms_reorder_beams(*args)
     if rc:
         raise _lib.FmmsError(rc, "fmms_reorder_beams")
+    increment_version(states)  # as torch's own operations do: what autograd has saved of them is no longer there
 
 
 class BeamSearch:

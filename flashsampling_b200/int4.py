@@ -9,6 +9,7 @@ bits per element are a quarter of the bf16 stream.  The result is that of the de
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .core import _refuse_gradients, _status_word
@@ -157,7 +158,8 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
         x2 = x2.contiguous()
     b = x2.shape[0]
     shape = x.shape[:-1] + (weight.rows,)
-    if out is None:
+    given = out is not None
+    if not given:
         out_dtype = out_dtype or x.dtype
         if out_dtype not in _DTYPES:
             raise TypeError("out_dtype must be bfloat16, float16 or float32")
@@ -186,6 +188,8 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
             rc = _launch(x2, stride, weight, b, out, out_stride, index)
     if rc:
         raise _lib.FmmsError(rc, "fmms_int4_linear")
+    if given:
+        increment_version(out)
     return out
 
 

@@ -1,4 +1,4 @@
-"""The operators around a decode step beside autograd: derivatives are refused."""
+"""The operators around a decode step beside autograd: derivatives are refused, writes into a caller's tensors are seen."""
 
 import pytest
 import torch
@@ -37,3 +37,33 @@ def test_tangents_are_refused(fs, batch):
                 call()
         fs.int4_linear(x, w, out=out)  # nothing carries a tangent
         fs.reorder_beams(logits[0], fs.beam_search_step(logits, scores).parents)
+
+
+@pytest.mark.parametrize("batch", [2, 12])
+def test_writes_raise_the_version(fs, batch):
+    w = _weight(fs)
+    x = torch.randn(batch, 64, device="cuda:0").bfloat16()
+    out = torch.empty(batch, 48, device="cuda:0")
+    before = out._version
+    fs.int4_linear(x, w, out=out)
+    assert out._version > before
+    parents = torch.tensor([[1, 0, 3, 2]], device="cuda:0")
+    states = [torch.randn(4, 8, device="cuda:0") for _ in range(3)]
+    losses = [(s * torch.ones_like(s).requires_grad_()).sum() for s in (*states, out)]
+    fs.reorder_beams(states, parents)
+    with torch.no_grad():
+        fs.int4_linear(x[:1], w, out=out[:1])
+    for loss in losses:  # each has saved a tensor that is another one now
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+
+
+def test_tensors_of_inference_mode_have_no_version(fs):
+    with torch.inference_mode():
+        w = _weight(fs)
+        x = torch.randn(3, 64, device="cuda:0").bfloat16()
+        state = torch.arange(8, device="cuda:0").view(4, 2)
+        out = fs.int4_linear(x, w, out=torch.empty(3, 48, device="cuda:0"))
+        fs.reorder_beams(state, torch.tensor([[1, 0, 3, 2]], device="cuda:0"))
+    assert torch.equal(out, fs.int4_linear(x, w, out_dtype=torch.float32))
+    assert state.tolist() == [[2, 3], [0, 1], [6, 7], [4, 5]]

@@ -29,7 +29,7 @@ class Int4Weight:
     ``16 tile + 8 + g`` (high nibble) of column ``64 chunk + 16 j + 8 b0 + 2 t + b1``.  ``scales`` (bf16 or fp16) and
     ``zeros`` (uint8, or ``None``: 8 everywhere) are ``[tiles, groups, 8, 2]``, row ``g`` and row ``8 + g`` next to
     each other.  A weight is ``(q - zero) * scale``.  What rows and columns beyond the weight hold does not matter.
-    The tensors' contents may change, the tensors themselves may not.
+    The tensors' contents may change, the tensors themselves may not: a call refuses a weight whose tensors have moved.
 
     ``Int4Weight.from_rows`` lays out plain codes, ``Int4Weight.quantize`` rounds a floating-point weight.
     """
@@ -69,6 +69,14 @@ class Int4Weight:
 
     def __reduce__(self):
         return (Int4Weight, (self.qweight, self.scales, self.zeros, self.rows, self.cols))
+
+    def _call_args(self) -> tuple:
+        """What a call passes on, if the tensors still lie where they did (``t.data = ...`` and ``t.resize_`` move them)."""
+        args = self._args
+        if (self.qweight.data_ptr() != args[0] or self.scales.data_ptr() != args[1]
+                or (self.zeros is not None and self.zeros.data_ptr() != args[3])):
+            raise RuntimeError("a tensor of this Int4Weight has got other memory since: make a new Int4Weight")
+        return args
 
     @property
     def shape(self) -> tuple[int, int]:
@@ -194,7 +202,7 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
 
 
 def _launch(x, stride, weight, b, out, out_stride, index):
-    qw, scales, scale_dtype, zeros, rows, cols, group = weight._args
+    qw, scales, scale_dtype, zeros, rows, cols, group = weight._call_args()
     key = (rows, cols, group, b)
     nbytes = _ws_bytes.get(key)
     if nbytes is None:

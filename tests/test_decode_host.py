@@ -286,3 +286,22 @@ def test_dynamic_shared_memory_has_one_alignment_per_name():
         for align, name in re.findall(r"extern __shared__ (?:__align__\((\d+)\) )?[\w ]+? (\w+)\[\]", unit(source.resolve(), set())):
             found.setdefault(name, set()).add(align)
         assert found and all(len(aligns) == 1 for aligns in found.values()), (source.name, found)
+
+
+@pytest.mark.parametrize("name", ["qweight", "scales", "zeros"])
+def test_a_weight_whose_tensors_moved_is_refused(name):
+    for move in (lambda t: setattr(t, "data", t.clone()), lambda t: t.resize_(64, *t.shape[1:]), lambda t: t.untyped_storage().resize_(0)):
+        w = fs.Int4Weight.from_rows(*_codes(20, 128, 64, True))
+        assert w._call_args() == (w.qweight.data_ptr(), w.scales.data_ptr(), _lib.BF16, w.zeros.data_ptr(), 20, 128, 64)
+        getattr(w, name).fill_(1)  # contents may change
+        assert w._call_args() is w._args
+        old = getattr(w, name).data  # keeps the memory, so that no other tensor gets its address
+        move(getattr(w, name))
+        if getattr(w, name).data_ptr() != w._args[("qweight", "scales", "", "zeros").index(name)]:
+            with pytest.raises(RuntimeError, match="make a new Int4Weight"):
+                w._call_args()
+        else:
+            raise AssertionError("the tensor has not moved")
+        del old
+    symmetric = fs.Int4Weight.from_rows(*_codes(20, 128, 64, False))
+    assert symmetric._call_args()[3] is None

@@ -333,6 +333,8 @@ int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void*
     m.scale_off = mp.scale_off;
     m.idesc = (1u << 4) | ((uint32_t)(mp.n >> 3) << 17) | ((128u >> 4) << 24);  // fp32 sums of fp16 products, 128 x n
     m.status_dev = status_dev;
+    m.wait_ns = kWaitLimitNs;
+    m.x_limit = 0x7fffffff;
     return zeros ? int4_mma_launch_group<true>(m, mp, group, dev, num_sms, staged, exponents, s)
                  : int4_mma_launch_group<false>(m, mp, group, dev, num_sms, staged, exponents, s);
   }

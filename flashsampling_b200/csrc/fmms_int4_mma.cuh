@@ -62,6 +62,8 @@ struct Int4MmaParams {
   int x_stages, ring_off, scale_off;
   uint32_t idesc;
   int* status_dev;
+  unsigned long long wait_ns;  // how long a wait may take
+  int x_limit;                 // steps of x that a CTA fetches, at most: fewer than there are makes the waits for them run out
 };
 
 // One CTA per row of x.
@@ -345,7 +347,7 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
       asm volatile("cp.async.wait_group %0;" ::"n"(kInt4MmaRing - 2) : "memory");
       if constexpr (ZP) __syncwarp();  // zeros were copied by other lanes
       const uint8_t* src = ring + slot * kSlot;
-      if (round > 0) mbar_wait(&done[at_slot], (uint32_t)(round - 1) & 1u, abort_flag, p.status_dev);
+      if (round > 0) mbar_wait(&done[at_slot], (uint32_t)(round - 1) & 1u, abort_flag, p.status_dev, p.wait_ns);
       tc_fence_after();
       const uint32_t at = tmem + lanes + at_slot * (kStepU * 64) + half * 32;
 #pragma unroll
@@ -425,7 +427,6 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
     int slot = 0, d = 0, dround = 0;
 #pragma unroll 1
     for (int block = 0; block < blocks; ++block) {
-      const bool there = t_count - block * 8 - quad > tile_of * 4;
       float2 tot[kCols / 2];
 #pragma unroll
       for (int i = 0; i < kCols / 2; ++i) tot[i] = make_float2(0.f, 0.f);
@@ -439,7 +440,8 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
         for (int gi = 0; gi < kStepG; ++gi)
           s[gi] = half_bits_to_float(reinterpret_cast<const uint16_t*>(ring + slot * kScaleBytes)[tile_of * (kStepG * 16) + gi * 16 + place], q.s_bf16);
         if (++slot == kInt4MmaScaleRing) slot = 0;
-        mbar_wait(&done[d], (uint32_t)dround & 1u, abort_flag, p.status_dev);
+        mbar_wait(&done[d], (uint32_t)dround & 1u, abort_flag, p.status_dev, p.wait_ns);
+        __syncwarp();
         tc_fence_after();
         const int groups = GR == kInt4Unit ? min(kStepU, q.all_units - unit) : min(kStepG, q.groups - unit * kGroups);
         const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16) + kSumAt + d * (kStepG * NC) + first_col;
@@ -464,25 +466,30 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
           ++dround;
         }
       }
+      // (after a wait that ran out, here or elsewhere, what has been added up need not be sums)
+      const bool there = t_count - block * 8 - quad > tile_of * 4 && !*abort_flag;
       const int v = (t_begin + block * 8 + quad + tile_of * 4) * kInt4Tile + r16;
 #pragma unroll
       for (int i = 0; i < kCols; ++i) {
         const float y = ((i & 1) ? tot[i / 2].y : tot[i / 2].x) * __shfl_sync(0xffffffffu, down0, i) * __shfl_sync(0xffffffffu, down1, i);
         if (there && v < q.V && first_col + i < nb) int4_store(q, pass * p.n + first_col + i, v, y);
       }
+      if (__any_sync(0xffffffffu, *abort_flag)) break;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kInt4MmaWeightWarps + kInt4MmaSumWarps) {
     // ------------------------------ products ------------------------------
     // The whole warp runs the loop, so that addresses stay in uniform registers; one elected lane issues.
-    int a = 0, around = 0, x = 0, xround = 0, unit = 0;
+    int a = 0, around = 0, x = 0, xround = 0, unit = 0, issued = 0;
 #pragma unroll 1
-    for (int step = 0; step < steps; ++step) {
+    for (; issued < steps; ++issued) {
       // three conditions at once: lanes 0 mod 3 wait for x, 1 for the accumulators, 2 for the weights
       const int what = lane % 3;
+      bool ok = true;
       if (what != 1 || around > 0)
-        mbar_wait(what == 0 ? &x_full[x] : what == 1 ? &d_empty[a] : &a_full[a],
-                  (uint32_t)(what == 0 ? xround : what == 1 ? around - 1 : around) & 1u, abort_flag, p.status_dev);
-      __syncwarp();
+        ok = mbar_wait(what == 0 ? &x_full[x] : what == 1 ? &d_empty[a] : &a_full[a],
+                       (uint32_t)(what == 0 ? xround : what == 1 ? around - 1 : around) & 1u, abort_flag, p.status_dev, p.wait_ns);
+      if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       const int groups = GR == kInt4Unit ? min(kStepU, q.all_units - unit) : min(kStepG, q.groups - unit * kGroups);
       const uint64_t desc = umma_smem_desc(smem_u32(smem) + x * kXBytes);
@@ -513,18 +520,18 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
       }
       unit += kStepU;
       if (unit >= q.all_units) unit = 0;
-      if (*abort_flag) break;
     }
-    // the last commit has to arrive while the CTA is still there
-    mbar_wait(&x_empty[(steps - 1) % p.x_stages], (uint32_t)((steps - 1) / p.x_stages) & 1u, abort_flag, p.status_dev);
+    // the products that were issued have to end, and the last commit to arrive, while the CTA and its tensor memory are there
+    if (issued > 0 && !mbar_wait_plain(&x_empty[(issued - 1) % p.x_stages], (uint32_t)((issued - 1) / p.x_stages) & 1u, kWaitLimitNs) && p.status_dev)
+      atomicExch(p.status_dev, kErrTimeout);
   } else if (lane == 0) {
     // ------------------------------ x ------------------------------
     griddep_wait();
     const uint8_t* src = p.staged + (size_t)pass * row_steps * kXBytes;
     int x = 0, round = 0, at = 0, issued = 0;
 #pragma unroll 1
-    for (int step = 0; step < steps; ++step) {
-      if (round > 0 && !mbar_wait(&x_empty[x], (uint32_t)(round - 1) & 1u, abort_flag, p.status_dev)) break;
+    for (int step = 0; step < min(steps, p.x_limit); ++step) {
+      if (round > 0 && !mbar_wait(&x_empty[x], (uint32_t)(round - 1) & 1u, abort_flag, p.status_dev, p.wait_ns)) break;
       mbar_arrive_expect_tx(&x_full[x], (uint32_t)kXBytes);
       bulk_load(smem + x * kXBytes, src + (size_t)at * kXBytes, (uint32_t)kXBytes, &x_full[x]);
       ++issued;
@@ -534,12 +541,11 @@ __global__ void __launch_bounds__(kInt4MmaThreads, 1) int4_mma_kernel(const Int4
         ++round;
       }
     }
-    // a wait ran out somewhere: give copies still in flight a bounded chance to land before the CTA's memory is reused
-    if (*abort_flag)
-      for (int i = 0; i < min(issued, p.x_stages); ++i) {
-        const int last = ((issued - 1 - i) / p.x_stages) * p.x_stages + i;
-        mbar_wait_plain(&x_full[i], (uint32_t)(last / p.x_stages) & 1u, 100000000ull);
-      }
+    // copies land before the CTA's memory is reused, also when a wait ran out and no product asks for them
+    for (int i = 0; i < min(issued, p.x_stages); ++i) {
+      const int last = ((issued - 1 - i) / p.x_stages) * p.x_stages + i;
+      mbar_wait_plain(&x_full[i], (uint32_t)(last / p.x_stages) & 1u, kWaitLimitNs);
+    }
   }
   tc_fence_before();
   __syncthreads();

@@ -380,7 +380,8 @@ int fmms_static_reset(void* stream);
  *   out          [B, V] bf16, fp16 or fp32, rows `out_stride` elements apart; written once, nothing else is touched
  *   workspace    fmms_query_int4_workspace() bytes, 16-byte aligned (0 bytes, and NULL, for up to eight rows that fit shared
  *                memory); holds nothing between calls, need not be zeroed, and must not be used by two calls at once
- *   status_dev   an int, or NULL: set to FMMS_ERR_TIMEOUT when a wait between the warps of a kernel ran out (as in the other calls)
+ *   status_dev   an int, or NULL: set to FMMS_ERR_TIMEOUT when a wait between the warps of a kernel ran out (as in the other
+ *                calls); outputs that were not there yet are then left as they were
  *
  * Sums are fp32.  x is brought to fp16 with an exact power of two per row: values below 2^-28 of a row's largest lose bits
  * beyond 2^-39 of it in calls of up to eight rows, values below 2^-24 (bf16; 2^-21 for fp16) bits beyond 2^-32 in larger ones.

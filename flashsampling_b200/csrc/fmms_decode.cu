@@ -17,6 +17,8 @@ namespace fmms {
 constexpr int kDecodeMaxDevices = 16;
 constexpr int kInt4SmemLimit = 230000;  // of 232448 bytes a CTA may have; the rest: static shared memory and alignment
 
+static bool on_boundary(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (unsigned)bytes == 0; }
+
 static int decode_num_sms(int* dev_out, int* sms_out) {
   static std::atomic<int> sms[kDecodeMaxDevices];
   int dev = 0;
@@ -280,6 +282,7 @@ int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void*
       out_dtype < FMMS_BF16 || out_dtype > FMMS_F32)
     return FMMS_ERR_BAD_ARG;
   if (x_stride < D || out_stride < V) return FMMS_ERR_BAD_ARG;
+  if (!on_boundary(x, 2) || !on_boundary(out, out_dtype == FMMS_F32 ? 4 : 2) || !on_boundary(status_dev, 4)) return FMMS_ERR_BAD_ARG;
   if (!int4_group_ok(group, D)) return FMMS_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(qweight) | reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(zeros)) & 15)
     return FMMS_ERR_UNSUPPORTED;
@@ -363,7 +366,9 @@ int fmms_beam_step(const void* logits, int dtype, long long stride_r, long long 
   if (!logits || !scores || !out_scores || !out_tokens || !out_parents) return FMMS_ERR_BAD_ARG;
   if (R <= 0 || K <= 0 || V <= 0 || N <= 0 || dtype < FMMS_BF16 || dtype > FMMS_F32) return FMMS_ERR_BAD_ARG;
   if (pad_token < 0 || pad_token >= V || N > (long long)K * V) return FMMS_ERR_BAD_ARG;
-  if (reinterpret_cast<uintptr_t>(logits) % beam_element_bytes(dtype)) return FMMS_ERR_BAD_ARG;
+  if (!on_boundary(logits, beam_element_bytes(dtype)) || !on_boundary(scores, 4) || !on_boundary(out_scores, 4) || !on_boundary(out_tokens, 8) ||
+      !on_boundary(out_parents, 8))
+    return FMMS_ERR_BAD_ARG;
   if (N > kBeamMaxN || K > kBeamMaxK || (long long)K * V >= (1ll << 31) || (long long)R * K > 65535) return FMMS_ERR_UNSUPPORTED;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < beam_workspace(R, K, V, N, dtype))
     return FMMS_ERR_WORKSPACE;
@@ -404,6 +409,7 @@ int fmms_beam_step(const void* logits, int dtype, long long stride_r, long long 
 int fmms_reorder_beams(const fmms_beam_state_t* states, int n_states, const void* parents, int parents_bytes, int R, int K,
                        const int* lengths, void* stream) {
   if (!states || n_states <= 0 || !parents || R <= 0 || K <= 0 || (parents_bytes != 4 && parents_bytes != 8)) return FMMS_ERR_BAD_ARG;
+  if (!on_boundary(parents, parents_bytes) || !on_boundary(lengths, 4)) return FMMS_ERR_BAD_ARG;
   if (K > kReorderMaxBeams) return FMMS_ERR_UNSUPPORTED;
   for (int i = 0; i < n_states; ++i) {
     const fmms_beam_state_t& s = states[i];

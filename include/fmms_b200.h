@@ -362,7 +362,7 @@ int fmms_static_reset(void* stream);
  * head only (core.py:224-348).
  */
 
-/* element types of these operators */
+/* element types of these operators; a pointer that is not on a multiple of its element's size is FMMS_ERR_BAD_ARG */
 #define FMMS_BF16 0
 #define FMMS_F16 1
 #define FMMS_F32 2

@@ -305,3 +305,26 @@ def test_a_weight_whose_tensors_moved_is_refused(name):
         del old
     symmetric = fs.Int4Weight.from_rows(*_codes(20, 128, 64, False))
     assert symmetric._call_args()[3] is None
+
+
+def test_c_entry_points_refuse_pointers_off_their_types(lib):
+    """An element that does not lie on a multiple of its size would be a misaligned access on the GPU."""
+    p = 4096  # never dereferenced
+
+    def int4(x=p, out=p, out_dtype=0, status=None, batch=2):
+        return lib.fmms_int4_linear(x, 0, 64, p, p, 0, None, 100, 64, 64, batch, out, out_dtype, 100, p, 1 << 30, status, None)
+
+    for batch in (2, 20):
+        for kw in (dict(x=p + 1), dict(out=p + 1), dict(out=p + 2, out_dtype=2), dict(out=p + 1, out_dtype=1), dict(status=p + 2)):
+            assert int4(batch=batch, **kw) == _lib.ERR_BAD_ARG, kw
+
+    def step(scores=p, os=p, ot=p, op=p):
+        return lib.fmms_beam_step(p, 0, 4000, 1000, scores, None, 0, 2, 4, 1000, 8, os, ot, op, p, 1 << 20, None)
+
+    for kw in (dict(scores=p + 2), dict(os=p + 1), dict(ot=p + 4), dict(op=p + 4)):
+        assert step(**kw) == _lib.ERR_BAD_ARG, kw
+
+    st = (_lib.FmmsBeamState * 1)()
+    st[0].data, st[0].beam_stride, st[0].seg_bytes, st[0].outer[0], st[0].outer[1] = p, 64, 64, 1, 1
+    for parents, size, lengths in ((p + 4, 8, None), (p + 2, 4, None), (p, 8, p + 2)):
+        assert lib.fmms_reorder_beams(st, 1, parents, size, 2, 4, lengths, None) == _lib.ERR_BAD_ARG

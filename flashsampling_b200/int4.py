@@ -143,7 +143,7 @@ class Int4Weight:
 def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype | None = None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T`` for bf16 or fp16 ``x [..., cols]``: ``[..., rows]`` in ``out_dtype`` (bf16, fp16 or fp32; default
-    the type of ``x``), or into ``out``.
+    the type of ``x``), or into ``out``, which must not share memory with ``x``.
 
     Made for the few rows of a decode step: up to eight rows cost little more than the weight's stream, 16 to 32 rows one
     and a half to two times that, and more than 64 (32 for groups of 32 columns) stream the weight more than once.  Rows of
@@ -188,6 +188,8 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
     if b == 0:
         return out
     stride = x2.stride(0) if b > 1 else max(x2.stride(0), weight.cols)
+    if given and _rows_meet(x2, stride, out, out_stride, b, weight):
+        raise ValueError("out must not share memory with x: rows of x are still read while others are written")
     index = dev.index
     if torch._C._cuda_getDevice() == index:
         rc = _launch(x2, stride, weight, b, out, out_stride, index)
@@ -199,6 +201,19 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
     if given:
         increment_version(out)
     return out
+
+
+def _rows_meet(x, stride, out, out_stride, b, weight) -> bool:
+    """Whether the rows that are read and those that are written have bytes in common (side by side in one buffer: no)."""
+    ex, eo = x.element_size(), out.element_size()
+    pitch, pitch_out, width, width_out = stride * ex, out_stride * eo, weight.cols * ex, weight.rows * eo
+    apart = out.data_ptr() - x.data_ptr()
+    if apart >= (b - 1) * pitch + width or -apart >= (b - 1) * pitch_out + width_out:
+        return False
+    if b == 1 or pitch != pitch_out:
+        return True
+    apart %= pitch
+    return apart < width or apart + width_out > pitch
 
 
 def _launch(x, stride, weight, b, out, out_stride, index):

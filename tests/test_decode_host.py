@@ -328,3 +328,37 @@ def test_c_entry_points_refuse_pointers_off_their_types(lib):
     st[0].data, st[0].beam_stride, st[0].seg_bytes, st[0].outer[0], st[0].outer[1] = p, 64, 64, 1, 1
     for parents, size, lengths in ((p + 4, 8, None), (p + 2, 4, None), (p, 8, p + 2)):
         assert lib.fmms_reorder_beams(st, 1, parents, size, 2, 4, lengths, None) == _lib.ERR_BAD_ARG
+
+
+def test_rows_that_share_memory_are_found():
+    from types import SimpleNamespace
+
+    from flashsampling_b200.int4 import _rows_meet
+
+    g = torch.Generator().manual_seed(0)
+
+    def r(lo, hi):
+        return int(torch.randint(lo, hi, (1,), generator=g))
+
+    found = set()
+    for _ in range(2000):
+        buf = torch.zeros(400, dtype=torch.bfloat16)
+        b, cols, rows = r(1, 5), r(1, 12), r(1, 12)
+        sx = cols + r(0, 20)
+        so = sx if r(0, 2) and sx >= rows else rows + r(0, 20)
+        x = buf.as_strided((b, cols), (sx, 1), r(0, 150))
+        out = buf.as_strided((b, rows), (so, 1), r(0, 150))
+        marks = torch.zeros(400, dtype=torch.int32)
+        marks.as_strided(x.shape, x.stride(), x.storage_offset()).add_(1)
+        want = bool((marks.as_strided(out.shape, out.stride(), out.storage_offset()) > 0).any())
+        got = _rows_meet(x, sx, out, so, b, SimpleNamespace(rows=rows, cols=cols))
+        assert got or not want  # nothing shared is missed
+        if b == 1 or (sx == so and want):
+            assert got == want
+        found.add((want, got))
+    assert {(False, False), (True, True)} <= found
+    # x and out side by side in one buffer, and x over itself
+    buf = torch.zeros(6, 30, dtype=torch.bfloat16)
+    side = SimpleNamespace(rows=14, cols=16)
+    assert not _rows_meet(buf[:, :16], 30, buf[:, 16:], 30, 6, side) and not _rows_meet(buf[:, 14:], 30, buf[:, :14], 30, 6, side)
+    assert _rows_meet(buf[:, :16], 30, buf[:, 15:29], 30, 6, side) and _rows_meet(buf[:, :16], 30, buf[:, :14], 30, 6, side)

@@ -422,3 +422,17 @@ def test_status_word_of_a_process_whose_first_calls_are_captured(fs):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", _STATUS], cwd=root, capture_output=True, text=True, timeout=240)
     assert done.returncode == 0 and "status kept" in done.stdout, done.stdout[-500:] + done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("batch", [1, 6, 20])
+def test_out_over_x_is_refused(fs, batch):
+    w = _weight(fs, 256, 256, 64, False)
+    x = _x(batch, 256, torch.bfloat16)
+    want = fs.int4_linear(x, w)
+    buf = torch.zeros(batch, 600, dtype=torch.bfloat16, device=_dev())
+    buf[:, :256] = x
+    for out in (buf[:, :256], buf[:, 128:384], buf[:, 255:511]):
+        with pytest.raises(ValueError, match="share memory"):
+            fs.int4_linear(buf[:, :256], w, out=out)
+    fs.int4_linear(buf[:, :256], w, out=buf[:, 256:512])  # side by side
+    assert torch.equal(buf[:, 256:512], want) and torch.equal(buf[:, :256], x)

@@ -315,7 +315,7 @@ class BeamSearch:
         its length to the power ``length_penalty``; the length counts up to and with ``eos_token``."""
         tokens = self.tokens[:, :self.steps].view(self.requests, self.beams, -1)
         length = torch.full_like(self.scores, float(max(1, self.steps)))
-        if self.eos_token is not None:
+        if self.eos_token is not None and self.steps:
             ends = tokens == self.eos_token
             length = torch.where(ends.any(-1), ends.to(torch.int8).argmax(-1).float() + 1, length)
         ranked = self.scores / length**length_penalty

@@ -362,3 +362,14 @@ def test_rows_that_share_memory_are_found():
     side = SimpleNamespace(rows=14, cols=16)
     assert not _rows_meet(buf[:, :16], 30, buf[:, 16:], 30, 6, side) and not _rows_meet(buf[:, 14:], 30, buf[:, :14], 30, 6, side)
     assert _rows_meet(buf[:, :16], 30, buf[:, 15:29], 30, 6, side) and _rows_meet(buf[:, :16], 30, buf[:, :14], 30, 6, side)
+
+
+@pytest.mark.parametrize("eos", [None, 3])
+def test_best_before_the_first_step_is_empty(eos):
+    search = fs.BeamSearch.__new__(fs.BeamSearch)  # its tensors without a GPU
+    search.requests, search.beams, search.max_steps, search.eos_token, search.pad_token, search.steps = 2, 3, 5, eos, 0, 0
+    search.tokens = torch.zeros(6, 5, dtype=torch.int64)
+    search.scores = torch.tensor([[0.0, -torch.inf, -torch.inf]]).repeat(2, 1)
+    search.finished = torch.zeros(2, 3, dtype=torch.bool)
+    tokens, scores = search.best(length_penalty=1.0)
+    assert tokens.shape == (2, 0) and scores.tolist() == [0.0, 0.0]

@@ -167,6 +167,8 @@ def _describe(s: torch.Tensor, dim: int, length_dim: int | None, R: int, K: int,
     blocks = _merge_dims([(sizes[i], strides[i]) for i in range(s.ndim) if i != dim and i < first])
     if len(blocks) > 2:
         raise ValueError("a state's dimensions around the beams must form at most two even sequences")
+    if any(size >= 1 << 31 for size, _ in blocks):
+        raise ValueError("a state's dimensions around the beams must be below 2^31 blocks each")
     while len(blocks) < 2:
         blocks.insert(0, (1, 0))
     desc.data = s.data_ptr()

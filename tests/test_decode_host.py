@@ -373,3 +373,13 @@ def test_best_before_the_first_step_is_empty(eos):
     search.finished = torch.zeros(2, 3, dtype=torch.bool)
     tokens, scores = search.best(length_penalty=1.0)
     assert tokens.shape == (2, 0) and scores.tolist() == [0.0, 0.0]
+
+
+def test_description_refuses_what_its_fields_cannot_hold():
+    """Two beams of one byte each behind 2^32 + 5 blocks: 32 bits would make five of them."""
+    desc = _lib.FmmsBeamState()
+    for blocks in ((1 << 32) + 5, 1 << 31):
+        with pytest.raises(ValueError, match="2\\^31"):
+            beam._describe(torch.empty(blocks, 2, dtype=torch.uint8, device="meta"), 1, None, 1, 2, desc, False)
+    beam._describe(torch.empty((1 << 31) - 1, 2, dtype=torch.uint8, device="meta"), 1, None, 1, 2, desc, False)
+    assert desc.outer[1] == (1 << 31) - 1

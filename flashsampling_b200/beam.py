@@ -13,6 +13,7 @@ import math
 from typing import NamedTuple, Sequence
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _lib
@@ -86,7 +87,8 @@ def beam_search_step(
         raise ValueError(f"pad_token must be one of the {V} tokens")
     if V > 1 and logits.stride(-1) != 1:
         raise ValueError("the logits of a row must be consecutive")
-    _refuse_gradients("beam_search_step", logits, scores)
+    if logits.requires_grad or scores.requires_grad or forward_ad._current_level >= 0:
+        _refuse_gradients("beam_search_step", logits, scores)
     if not scores.is_contiguous():
         scores = scores.contiguous()
     done = None
@@ -167,10 +169,10 @@ def _describe(s: torch.Tensor, dim: int, length_dim: int | None, R: int, K: int,
     blocks = _merge_dims([(sizes[i], strides[i]) for i in range(s.ndim) if i != dim and i < first])
     if len(blocks) > 2:
         raise ValueError("a state's dimensions around the beams must form at most two even sequences")
-    if any(size >= 1 << 31 for size, _ in blocks):
-        raise ValueError("a state's dimensions around the beams must be below 2^31 blocks each")
     while len(blocks) < 2:
         blocks.insert(0, (1, 0))
+    if blocks[0][0] >= 1 << 31 or blocks[1][0] >= 1 << 31:
+        raise ValueError("a state's dimensions around the beams must be below 2^31 blocks each")
     desc.data = s.data_ptr()
     desc.beam_stride = strides[dim] * es
     desc.outer_stride[0], desc.outer_stride[1] = blocks[0][1] * es, blocks[1][1] * es
@@ -212,11 +214,12 @@ def reorder_beams(
         lengths = lengths.contiguous()
     parents = parents.contiguous()
     descs = (_lib.FmmsBeamState * max(1, len(states)))()
-    n, seen = 0, set()
+    n, seen, dual = 0, set(), forward_ad._current_level >= 0
     for s in states:
         if s.device != dev:
             raise ValueError(f"a state is on {s.device}, parents on {dev}")
-        _refuse_gradients("reorder_beams (in place)", s)
+        if s.requires_grad or dual:
+            _refuse_gradients("reorder_beams (in place)", s)
         if s.is_complex() or s.is_sparse or s.is_quantized:
             raise TypeError("states must be plain dense tensors")
         d = dim + s.ndim if dim < 0 else dim

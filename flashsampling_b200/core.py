@@ -101,9 +101,8 @@ def _status_word(device: torch.device) -> torch.Tensor | None:
 
 def _refuse_gradients(where: str, *tensors: torch.Tensor) -> None:
     """Raise where autograd would want to go through one of ``tensors``, backward or forward."""
-    for t in tensors:
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{where} has no backward pass: call it under torch.no_grad()")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{where} has no backward pass: call it under torch.no_grad()")
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError(f"{where} has no forward-mode derivative, and a tensor carries a tangent")
 

@@ -9,6 +9,7 @@ bits per element are a quarter of the bf16 stream.  The result is that of the de
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _lib
@@ -160,7 +161,8 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
     dev = weight.qweight.device
     if x.device != dev:
         raise ValueError(f"x is on {x.device}, the weight on {dev}")
-    _refuse_gradients("int4_linear", x)
+    if x.requires_grad or forward_ad._current_level >= 0:
+        _refuse_gradients("int4_linear", x)
     x2 = x if x.ndim == 2 else x.reshape(-1, weight.cols)
     if x2.stride(1) != 1 or x2.stride(0) < weight.cols:
         x2 = x2.contiguous()
@@ -184,7 +186,8 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
             raise ValueError("out must have consecutive rows of consecutive elements")
         if out.requires_grad:
             raise RuntimeError("out must not require gradients")
-        _refuse_gradients("int4_linear", out)
+        if forward_ad._current_level >= 0:
+            _refuse_gradients("int4_linear", out)
     if b == 0:
         return out
     stride = x2.stride(0) if b > 1 else max(x2.stride(0), weight.cols)

@@ -91,6 +91,11 @@ static int int4_plan(Int4Plan& pl, int D, int group) {
 
 static bool int4_group_ok(int group, int D) { return (group == 32 || group == 64 || (group > 0 && group % kInt4Unit == 0)) && D % group == 0; }
 
+// Sizes whose sums and rounded multiples stay within 32 bits in plans and kernels; at most 65535 passes of eight-plus rows.
+static bool int4_sizes_ok(int V, int D, int group, int B) {
+  return V <= 0x7fffffff - (kInt4Tile - 1) && D <= (1 << 30) && B <= 65535 * int4_mma_max_n(group);
+}
+
 static size_t int4_workspace(const Int4Plan& pl, int V) {
   return pl.phases == 1 ? 0 : (size_t)((V + kInt4Tile - 1) / kInt4Tile) * 512;
 }
@@ -187,9 +192,14 @@ static int int4_mma_launch_group(const Int4MmaParams& p, const Int4MmaPlan& pl, 
 // ---- beam step ----------------------------------------------------------------------------------
 static int beam_element_bytes(int dtype) { return dtype == FMMS_F32 ? 4 : 2; }
 
+static bool beam_sizes_ok(int R, int K, int V, int N) {
+  return N <= kBeamMaxN && K <= kBeamMaxK && (long long)K * V < (1ll << 31) && (long long)R * K <= 65535;
+}
+
 // Vectors of a thread in a slice of a row, and slices of a row: as few slices as the list for their candidates allows,
-// but enough that the rows together make some four CTAs for each of the 148 SMs; not below four vectors, which the bound
-// is taken from.
+// but enough that the rows together make some four CTAs for each of a B200's 148 SMs (a constant, for the workspace's size is
+// asked for without a GPU, and sums must not depend on how many SMs there are); not below four vectors, which the bound is
+// taken from.
 static void beam_slices(int rows, int V, int dtype, int* iters, int* splits) {
   const long long per_iter = kBeamThreads * (16 / beam_element_bytes(dtype));
   const long long all = (V + per_iter - 1) / per_iter;
@@ -263,7 +273,7 @@ extern "C" {
 
 int fmms_query_int4_workspace(int V, int D, int group, int B, size_t* bytes) {
   if (!bytes || V <= 0 || D <= 0 || B <= 0) return FMMS_ERR_BAD_ARG;
-  if (!int4_group_ok(group, D)) return FMMS_ERR_UNSUPPORTED;
+  if (!int4_group_ok(group, D) || !int4_sizes_ok(V, D, group, B)) return FMMS_ERR_UNSUPPORTED;
   if (B > kInt4Rows) {
     *bytes = int4_mma_workspace(D, B, group);
     return FMMS_OK;
@@ -283,7 +293,7 @@ int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void*
     return FMMS_ERR_BAD_ARG;
   if (x_stride < D || out_stride < V) return FMMS_ERR_BAD_ARG;
   if (!on_boundary(x, 2) || !on_boundary(out, out_dtype == FMMS_F32 ? 4 : 2) || !on_boundary(status_dev, 4)) return FMMS_ERR_BAD_ARG;
-  if (!int4_group_ok(group, D)) return FMMS_ERR_UNSUPPORTED;
+  if (!int4_group_ok(group, D) || !int4_sizes_ok(V, D, group, B)) return FMMS_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(qweight) | reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(zeros)) & 15)
     return FMMS_ERR_UNSUPPORTED;
   const bool mma = B > kInt4Rows;
@@ -295,7 +305,6 @@ int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void*
   else
     rc = int4_plan(pl, D, group);
   if (rc != kOk) return rc;
-  if (mma && mp.passes > 65535) return FMMS_ERR_UNSUPPORTED;  // two to four million rows of x
   const size_t need = mma ? int4_mma_workspace(D, B, group) : int4_workspace(pl, V);
   if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need)) return FMMS_ERR_WORKSPACE;
   int dev = 0, num_sms = 0;
@@ -355,7 +364,7 @@ int fmms_int4_linear(const void* x, int x_dtype, long long x_stride, const void*
 
 int fmms_query_beam_workspace(int R, int K, int V, int N, int dtype, size_t* bytes) {
   if (!bytes || R <= 0 || K <= 0 || V <= 0 || N <= 0 || dtype < FMMS_BF16 || dtype > FMMS_F32) return FMMS_ERR_BAD_ARG;
-  if (N > kBeamMaxN || K > kBeamMaxK) return FMMS_ERR_UNSUPPORTED;
+  if (!beam_sizes_ok(R, K, V, N)) return FMMS_ERR_UNSUPPORTED;
   *bytes = beam_workspace(R, K, V, N, dtype);
   return FMMS_OK;
 }
@@ -369,7 +378,7 @@ int fmms_beam_step(const void* logits, int dtype, long long stride_r, long long 
   if (!on_boundary(logits, beam_element_bytes(dtype)) || !on_boundary(scores, 4) || !on_boundary(out_scores, 4) || !on_boundary(out_tokens, 8) ||
       !on_boundary(out_parents, 8))
     return FMMS_ERR_BAD_ARG;
-  if (N > kBeamMaxN || K > kBeamMaxK || (long long)K * V >= (1ll << 31) || (long long)R * K > 65535) return FMMS_ERR_UNSUPPORTED;
+  if (!beam_sizes_ok(R, K, V, N)) return FMMS_ERR_UNSUPPORTED;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < beam_workspace(R, K, V, N, dtype))
     return FMMS_ERR_WORKSPACE;
   int dev = 0, num_sms = 0;

@@ -385,6 +385,7 @@ int fmms_static_reset(void* stream);
  *
  * Sums are fp32.  x is brought to fp16 with an exact power of two per row: values below 2^-28 of a row's largest lose bits
  * beyond 2^-39 of it in calls of up to eight rows, values below 2^-24 (bf16; 2^-21 for fp16) bits beyond 2^-32 in larger ones.
+ * Limits (else FMMS_ERR_UNSUPPORTED): V <= 2^31 - 16, D <= 2^30, B <= 65535 * 64 (groups of 32: 65535 * 32).
  * A row of x that is not finite gives a row that is not finite.  The order of additions is fixed: equal calls give equal
  * bits, and a row's result does not depend on the other rows of its call's batch as long as the number of rows stays
  * within 1-8, or above 8.

@@ -383,3 +383,26 @@ def test_description_refuses_what_its_fields_cannot_hold():
             beam._describe(torch.empty(blocks, 2, dtype=torch.uint8, device="meta"), 1, None, 1, 2, desc, False)
     beam._describe(torch.empty((1 << 31) - 1, 2, dtype=torch.uint8, device="meta"), 1, None, 1, 2, desc, False)
     assert desc.outer[1] == (1 << 31) - 1
+
+
+def test_c_entry_points_refuse_sizes_that_overflow(lib):
+    """Products and rounded multiples of 32-bit sizes: a query divided by R * K = 2^32 = 0, plans got negative step counts,
+    and a kernel's column index would have wrapped."""
+    big, n = 0x7FFFFFFF, ctypes.c_size_t()
+    for sizes in ((1 << 26, 64, 1000, 8), (big, 64, 1000, 8), (65536, 1, 1000, 8), (1, 64, 1 << 25, 8)):
+        assert lib.fmms_query_beam_workspace(*sizes, 0, ctypes.byref(n)) == _lib.ERR_UNSUPPORTED, sizes
+    assert lib.fmms_query_beam_workspace(65535, 1, 1000, 8, 0, ctypes.byref(n)) == 0
+
+    def both(V, D, group, B):
+        p = 4096  # never dereferenced
+        query = lib.fmms_query_int4_workspace(V, D, group, B, ctypes.byref(n))
+        call = lib.fmms_int4_linear(p, 0, D, p, p, 0, None, V, D, group, B, p, 0, max(V, 1), None, 0, None, None)
+        assert (query == _lib.ERR_UNSUPPORTED) == (call == _lib.ERR_UNSUPPORTED)
+        return query
+
+    for sizes in ((big, 64, 64, 1), (big - 14, 64, 64, 16), (100, big - 127 + 96, 32, 16), (100, (1 << 30) + 128, 128, 16), (100, (1 << 30) + 128, 128, 1),
+                  (100, 64, 64, big), (100, 64, 64, 65535 * 64 + 1), (100, 64, 32, 65535 * 32 + 1)):
+        assert both(*sizes) == _lib.ERR_UNSUPPORTED, sizes
+    for sizes in ((big - 15, 64, 64, 16), (100, 1 << 30, 128, 16), (100, 64, 64, 65535 * 64), (100, 64, 32, 65535 * 32)):
+        assert both(*sizes) == 0, sizes
+        assert 0 < n.value < 1 << 45

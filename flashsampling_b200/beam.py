@@ -181,6 +181,13 @@ def _describe(s: torch.Tensor, dim: int, length_dim: int | None, R: int, K: int,
     desc.step_bytes = step
 
 
+def _check_beams(R: int, K: int) -> None:
+    if K < 1 or K > 64:
+        raise ValueError("reorder_beams takes 1 to 64 beams")
+    if R * K >= 1 << 31:
+        raise ValueError("reorder_beams takes requests * beams < 2^31")
+
+
 def reorder_beams(
     states: torch.Tensor | Sequence[torch.Tensor],  # any type; dimension `dim` is [requests * beams]
     parents: torch.Tensor,  # [requests, beams] int64 or int32
@@ -201,8 +208,7 @@ def reorder_beams(
     if not parents.is_cuda or not all(s.is_cuda for s in states):
         raise RuntimeError("reorder_beams requires CUDA tensors (there is no CPU path)")
     R, K = parents.shape
-    if K < 1 or K > 64:
-        raise ValueError("reorder_beams takes 1 to 64 beams")
+    _check_beams(R, K)
     dev = parents.device
     if lengths is not None and length_dim is None:
         raise ValueError("lengths needs length_dim, the states' dimension of positions")

@@ -40,6 +40,8 @@ class Int4Weight:
     def __init__(self, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None, rows: int, cols: int):
         if rows < 1 or cols < 1:
             raise ValueError("an Int4Weight needs at least one row and one column")
+        if rows > (1 << 31) - 16 or cols > 1 << 30:
+            raise ValueError("an Int4Weight has at most 2^31 - 16 rows and 2^30 columns")
         tiles, chunks = -(-rows // 16), -(-cols // 64)
         if qweight.dtype != torch.uint8 or qweight.shape != (tiles, chunks, 512):
             raise ValueError(f"qweight must be uint8 [{tiles}, {chunks}, 512] for a [{rows}, {cols}] weight")
@@ -167,6 +169,8 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
     if x2.stride(1) != 1 or x2.stride(0) < weight.cols:
         x2 = x2.contiguous()
     b = x2.shape[0]
+    if b >= 1 << 31:
+        raise ValueError("int4_linear takes fewer than 2^31 rows of x")
     shape = x.shape[:-1] + (weight.rows,)
     given = out is not None
     if not given:

@@ -406,3 +406,15 @@ def test_c_entry_points_refuse_sizes_that_overflow(lib):
     for sizes in ((big - 15, 64, 64, 16), (100, 1 << 30, 128, 16), (100, 64, 64, 65535 * 64), (100, 64, 32, 65535 * 32)):
         assert both(*sizes) == 0, sizes
         assert 0 < n.value < 1 << 45
+
+
+def test_sizes_beyond_the_c_entry_points_are_refused(monkeypatch):
+    """ctypes passes a Python integer of more than 32 bits on without its upper half."""
+    with pytest.raises(ValueError, match="2\\^31"):
+        fs.Int4Weight(torch.empty(((1 << 32) + 16) // 16, 1, 512, dtype=torch.uint8, device="meta"),
+                      torch.empty(((1 << 32) + 16) // 16, 1, 8, 2, dtype=torch.bfloat16, device="meta"), None, (1 << 32) + 16, 32)
+    with pytest.raises(ValueError, match="2\\^31"):
+        beam._check_beams((1 << 31) + 1, 2)
+    with pytest.raises(ValueError, match="64 beams"):
+        beam._check_beams(3, 65)
+    beam._check_beams((1 << 25) - 1, 64)

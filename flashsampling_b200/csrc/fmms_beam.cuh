@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kBeamThreads, 5) beam_part_kernel(const BeamPa
   // A row is cut into vectors from its first element on, wherever it lies, so that rows with the same values have the
   // same sums to the last bit: equal totals of two beams are told apart by (beam, token) alone.  Copies are the 16 bytes on
   // boundaries.  Where a row begins `shift` elements behind one, vector v is the end of copy v and the beginning of copy v + 1,
-  // the next lane's, and two lanes of a warp fetch what follows its last vectors.  (64 x 8 x 128257 bf16, 16 candidates: 58 us
+  // the next lane's, and two lanes of a warp fetch what follows its last vectors.  (64 x 8 x 128257 bf16, 16 candidates: 59 us
   // instead of the 50 us of 128256.)  The last VE to 2 VE - 1 elements, so that no copy ends behind the row, are the last
   // slice's singles.
   const int shift = EVEN ? 0 : (int)(reinterpret_cast<uintptr_t>(x) & 15) / (int)sizeof(T);

@@ -2,8 +2,8 @@
 // fmms_int4.cuh, on the fifth-generation tensor cores.
 //
 // mma.sync takes eight cycles for a 16 x 16 x 8 product here, so that beyond eight rows the products and not the weight's
-// stream set its pace (151936 x 4096: 55 us for one row, 59 us for 8, 83 us for 16, 216 us for 32, where this kernel takes
-// 89 us and 106 us; 128256 x 8192 at 16 rows: 200 us and 143 us).  tcgen05.mma takes 128 weight
+// stream set its pace (151936 x 4096: 55 us for one row, 60 us for 8, 83 us for 16, 216 us for 32, where this kernel takes
+// 88 us and 103 us; 128256 x 8192 at 16 rows: 200 us and 143 us).  tcgen05.mma takes 128 weight
 // rows against all rows of x at once, and it reads one operand from tensor memory: the weights go from registers there,
 // in the very layout the stored order is made for (tcgen05.st .16x128b places what a lane holds of a 16 x 16 operand), and
 // never through shared memory as fp16.

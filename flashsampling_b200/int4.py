@@ -148,10 +148,14 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, out_dtype: torch.dtype |
     """``x @ weight.T`` for bf16 or fp16 ``x [..., cols]``: ``[..., rows]`` in ``out_dtype`` (bf16, fp16 or fp32; default
     the type of ``x``), or into ``out``, which must not share memory with ``x``.
 
-    Made for the few rows of a decode step: up to eight rows cost little more than the weight's stream, 16 to 32 rows one
-    and a half to two times that, and more than 64 (32 for groups of 32 columns) stream the weight more than once.  Rows of
-    ``x`` may be strided.  Sums are fp32 and their order is fixed: a row of ``x`` gives the same bits in every batch of up
-    to eight rows, and in every larger one.  No gradients: the weight is for serving."""
+    Made for the few rows of a decode step.  In times of the weight's stream (at the rate of a plain copy) a large weight costs 1.1 for
+    one row and 1.2 for eight, with zero points and groups of 64 1.8 for five; 16 rows cost 1.7, 32 rows 2 (with groups
+    of 64 both above 3), 64 rows 3.4 to 5, and more than 64 (32 for groups of 32 columns) read the weight again for every 64.
+
+    Rows of ``x`` may be strided.  They are multiplied as fp16 after an exact power of two per row: bf16 values below 2^-28 of
+    their row's largest are rounded to 2^-39 of it, in batches of more than eight rows values below 2^-24 (fp16: 2^-21) to 2^-32
+    of it.  Sums are fp32 and their order is fixed: a row of ``x`` gives the same bits in every batch of up to eight rows, and in every
+    larger one.  No gradients: the weight is for serving."""
     if not isinstance(weight, Int4Weight):
         raise TypeError("weight must be an Int4Weight")
     if not (x.is_cuda and weight.qweight.is_cuda):

@@ -95,7 +95,7 @@ def _status_word(device: torch.device) -> torch.Tensor | None:
             with torch.cuda.stream(stream):
                 st = torch.zeros(1, dtype=torch.int32, device=device)
             stream.synchronize()
-        _status[device.index] = st
+        st = _status.setdefault(device.index, st)  # of two threads' words the first, whose address a call may have by now
     return st
 
 

@@ -121,10 +121,11 @@ def check_status(device: torch.device | None = None) -> None:
             continue
         code = int(st.item())
         if code != 0:
-            st.zero_()
-            for ws in _all_workspaces:
-                if ws.device.index == idx:
-                    ws.zero_()  # an aborted kernel may have left candidates behind
+            with torch.inference_mode():  # the tensors may have been made under it
+                st.zero_()
+                for ws in _all_workspaces:
+                    if ws.device.index == idx:
+                        ws.zero_()  # an aborted kernel may have left candidates behind
             raise _lib.FmmsError(code, "fused_mm_sample (device status word)")
 
 

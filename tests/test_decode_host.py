@@ -418,3 +418,17 @@ def test_sizes_beyond_the_c_entry_points_are_refused(monkeypatch):
     with pytest.raises(ValueError, match="64 beams"):
         beam._check_beams(3, 65)
     beam._check_beams((1 << 25) - 1, 64)
+
+
+def test_a_status_word_of_inference_mode_is_cleared(monkeypatch):
+    """A serving process makes the word and the workspaces under inference_mode and may check outside of it."""
+    from flashsampling_b200 import core
+
+    with torch.inference_mode():
+        word, workspace = torch.full((1,), _lib.ERR_TIMEOUT, dtype=torch.int32), torch.ones(8, dtype=torch.uint8)
+    monkeypatch.setattr(core, "_status", {None: word})  # (as a CPU tensor's device has it)
+    monkeypatch.setattr(core, "_all_workspaces", [workspace])
+    with pytest.raises(_lib.FmmsError):
+        fs.check_status()
+    assert int(word) == 0 and not bool(workspace.any())
+    fs.check_status()
